@@ -25,13 +25,10 @@
 // all roles leave their loops, the producer waits (bounded) for the loads it issued, the MMA thread
 // waits (bounded) for its last commit, and the TMEM is freed before the kernel returns; the host
 // reports the code as a runtime error.
-#include <cuda.h>
-
 #include <algorithm>
 #include <cstdlib>
-#include <mutex>
 
-#include "oztt_common.cuh"
+#include "tensor_core.cuh"
 
 namespace oztt {
 namespace gemm {
@@ -46,7 +43,6 @@ constexpr uint32_t TMEM_COLS = 2 * ACC_COLS;
 constexpr uint32_t NUM_THREADS = 192;
 constexpr uint32_t GROUP_M = 16;
 constexpr uint32_t SMEM_BYTES = STAGES * STAGE_BYTES + 256 + 1024;
-constexpr uint64_t TIMEOUT_NS = 2000000000ull;
 
 // Instruction descriptor of kind::i8: s32 accumulator, signed A and B, both K-major, N=256, M=128.
 constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((BN >> 3) << 17) | ((BM >> 4) << 24);
@@ -63,54 +59,6 @@ struct EpiConst {
     uint8_t out_a[OZTT_MAXOUT], out_b[OZTT_MAXOUT], out_g[OZTT_MAXOUT];
     uint16_t weight[OZTT_MAXOUT];
 };
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// Waits for the phase of `parity` to complete. Gives up when another role raised the abort flag or
-// after limit_ns (then records `code` and raises the flag). Returns true when the phase completed.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
-                                          int code, uint64_t limit_ns = TIMEOUT_NS) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = global_timer_ns();
-    for (uint32_t it = 1;; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 63) == 0) {
-            if (*abort_flag) return false;
-            if (global_timer_ns() - t0 > limit_ns) {
-                atomicOr(err, code);
-                *abort_flag = 1;
-                return false;
-            }
-        }
-    }
-}
-// Bounded wait used on the abort path only (ignores the abort flag).
-__device__ __forceinline__ void mbar_wait_drain(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
-    const uint64_t t0 = global_timer_ns();
-    while (!mbar_try_wait(bar, parity))
-        if (global_timer_ns() - t0 > limit_ns) return;
-}
 
 __device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint32_t dst, uint64_t* bar, int32_t c0,
                                             int32_t c1, int32_t c2) {
@@ -136,27 +84,6 @@ __device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t adesc, uint64_
         "l"(adesc), "l"(bdesc), "r"(IDESC), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(taddr)
-        : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
 // floor(a / m) for a < 2^31 with a precomputed (magic, shift) pair (round-up reciprocal method).
 __device__ __forceinline__ uint32_t udiv_small(uint32_t a, uint32_t magic, uint32_t shift) {
     return (__umulhi(a, magic) + a) >> shift;
@@ -485,23 +412,6 @@ constexpr uint32_t SMEM_BYTES = STAGES * STAGE_BYTES + 256 + 1024;
 constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((BN >> 3) << 17) | ((256u >> 4) << 24);
 constexpr uint64_t PEER_DRAIN_NS = 5000000ull;
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// The shared::cluster address of the same shared-memory offset in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t map_to(uint32_t smem_addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
 // TMA load into this CTA's shared memory, completing its bytes on a barrier of either CTA of the pair.
 __device__ __forceinline__ void tma_load_3d_pair(const CUtensorMap* map, uint32_t dst, uint32_t bar_cluster,
                                                  int32_t c0, int32_t c1, int32_t c2) {
@@ -519,12 +429,6 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t adesc, ui
         "l"(adesc), "l"(bdesc), "r"(IDESC), "r"(accumulate)
         : "memory");
 }
-// Arrives once on the barrier at `bar_cluster` (either CTA) when all MMAs issued so far have completed.
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_cluster)
-                 : "memory");
-}
-
 }  // namespace pair
 
 template <int MODE>
@@ -536,12 +440,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::NUM_THREADS, 1
     constexpr uint32_t BM = pair::BM, BN = pair::BN, BNH = pair::BNH, BK = pair::BK, UK = pair::UK;
     constexpr uint32_t STAGES = pair::STAGES, A_BYTES = pair::A_BYTES, STAGE_BYTES = pair::STAGE_BYTES;
     constexpr uint32_t ACC_COLS = pair::ACC_COLS, TMEM_COLS = pair::TMEM_COLS;
-    using pair::arrive_remote;
-    using pair::cluster_rank;
-    using pair::cluster_sync;
-    using pair::map_to;
     using pair::tma_load_3d_pair;
-    using pair::umma_commit_pair;
     using pair::umma_i8_pair;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -744,24 +643,6 @@ __global__ void __launch_bounds__(64) wait_probe_kernel(int* err_word, uint64_t 
 }
 
 // ---- host side -------------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-    });
-    if (!fn) throw Error(OZTT_ERUNTIME, "cuTensorMapEncodeTiled is not available from the CUDA driver");
-    return fn;
-}
-
 // 3-D map over S planes of rows x kp int8 (K innermost), box BK x box_rows x 1, 128-byte swizzle. The
 // planes lie plane_rows x pitch apart (plane_rows >= rows; a band of rows of taller planes), or rows x pitch;
 // rows lie pitch apart (pitch >= kp; a window of kp columns of wider rows), or kp.
