@@ -434,6 +434,42 @@ int oztt_set_option(int32_t option, int32_t value, char* err, size_t errlen);
 /* Reads an option's current value into *value. */
 int oztt_get_option(int32_t option, int32_t* value);
 
+/* ---- layers of networks: the product with its epilogue, and its gradients ---------------------------
+ * No counterpart in the reference, whose products are FP64. Device memory; BF16 or FP16 throughout (sums in 32
+ * bits, each result rounded once); asynchronous on `stream`, with scratch from the stream-ordered allocator.
+ * Any strides are taken; operands whose rows start on 16 bytes (and outputs whose rows start on 8) are read and
+ * written as they lie, others cost a copy of the operand. Outputs must not overlap operands, except y the
+ * residual it is computed from. A kernel that gives up a wait is reported by the next call (OZTT_ERUNTIME). */
+enum { OZTT_ACT_NONE = 0, OZTT_ACT_RELU = 1, OZTT_ACT_GELU = 2, OZTT_ACT_GELU_TANH = 3, OZTT_ACT_SILU = 4 };
+
+/* A matrix (or, with row_stride unused, a vector) by its strides in elements; data may be NULL where the
+ * operand is optional. A stride of 0 repeats a row or column (inputs only). */
+typedef struct oztt_view {
+    void* data;
+    int64_t row_stride, col_stride;
+} oztt_view;
+
+/* y = act(x w^T + bias) + residual: x m x k, w n x k, bias n (optional), residual m x n (optional), y m x n;
+ * pre (optional, m x n) receives x w^T + bias, which the backward pass of an activation needs. */
+typedef struct oztt_linear {
+    int32_t format;     /* OZTT_FMT_BF16 or OZTT_FMT_FP16 */
+    int32_t activation; /* OZTT_ACT_* */
+    uint64_t m, n, k;
+    oztt_view x, w, bias, residual, y, pre;
+} oztt_linear;
+int oztt_linear_forward(int device_id, const oztt_linear* args, void* stream, char* err, size_t errlen);
+
+/* The gradients, for dy m x n: dz = dy * act'(pre), then dx = dz w (m x k), dw = dz^T x (n x k), db = the sum of
+ * dz over its rows (n); each of dx, dw and db is computed when given. pre is needed with an activation, x for
+ * dw, w for dx. The gradient of the residual is dy itself. dz is rounded to the format once, except in db. */
+typedef struct oztt_linear_grad {
+    int32_t format;
+    int32_t activation;
+    uint64_t m, n, k;
+    oztt_view dy, pre, x, w, dx, dw, db;
+} oztt_linear_grad;
+int oztt_linear_backward(int device_id, const oztt_linear_grad* args, void* stream, char* err, size_t errlen);
+
 /* Number of SMs and compute capability of a device (0 on success). */
 int oztt_device_info(int device_id, int32_t* sm_count, int32_t* cc_major, int32_t* cc_minor);
 

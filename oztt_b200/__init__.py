@@ -12,6 +12,9 @@ throws ``std::invalid_argument``, ``RuntimeError`` for ``std::runtime_error``, `
 ``std::bad_alloc``. The lower-level functions (``ii_int8_plan``, ``ii_int8_run``, the stage calls)
 expose the backend seam and the individual kernels for tests and benchmarks.
 
+``linear`` and ``linear_backward`` (``layers.py``, on CUDA tensors of torch) are the 16-bit product of a
+network layer with its epilogue, and its gradients.
+
 There is no CPU fallback: every compute call goes to the CUDA kernels, and importing the module
 fails if the library has not been built.
 """
@@ -28,7 +31,7 @@ import numpy as np
 __all__ = [
     "Scheme", "Format", "Reconstruction", "Options", "DeviceOptions", "Info", "Context",
     "is_available", "format_name", "IIPlan", "ii_int8_plan", "ii_int8_run", "ii_int8_run_device",
-    "lib", "library_path",
+    "lib", "library_path", "linear", "linear_backward",
 ]
 
 _HERE = Path(__file__).resolve().parent
@@ -202,6 +205,8 @@ _SIGNATURES = {
     "oztt_resident_create": [ctypes.c_int, _I32, _P, _U64, _U64, _I32, ctypes.POINTER(_P), _ERR, _SZ],
     "oztt_resident_destroy": [_P],
     "oztt_resident_gemm": [_P, _P, _P, _I32, ctypes.POINTER(_COptions), ctypes.POINTER(_CInfo), _ERR, _SZ],
+    "oztt_linear_forward": [ctypes.c_int, _P, _P, _ERR, _SZ],
+    "oztt_linear_backward": [ctypes.c_int, _P, _P, _ERR, _SZ],
     "oztt_set_option": [_I32, _I32, _ERR, _SZ],
     "oztt_get_option": [_I32, ctypes.POINTER(_I32)],
     "oztt_is_available": [_I32],
@@ -246,9 +251,19 @@ def _lib() -> ctypes.CDLL:
     return _LIB
 
 
+# What lives in modules that need torch, imported on first use.
+_TORCH_NAMES = {"linear": "layers", "linear_backward": "layers"}
+
+
 def __getattr__(name: str):
     if name == "lib":
         return _lib()
+    if name in _TORCH_NAMES:
+        import importlib
+
+        value = getattr(importlib.import_module(f".{_TORCH_NAMES[name]}", __name__), name)
+        globals()[name] = value
+        return value
     raise AttributeError(name)
 
 

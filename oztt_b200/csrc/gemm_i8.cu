@@ -47,8 +47,6 @@ constexpr uint32_t SMEM_BYTES = STAGES * STAGE_BYTES + 256 + 1024;
 // Instruction descriptor of kind::i8: s32 accumulator, signed A and B, both K-major, N=256, M=128.
 constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((BN >> 3) << 17) | ((BM >> 4) << 24);
 
-enum ErrCode : int { ERR_WAIT_PRODUCER = 1, ERR_WAIT_MMA_FULL = 2, ERR_WAIT_MMA_EMPTY = 4, ERR_WAIT_EPILOGUE = 8 };
-
 struct EpiConst {
     uint32_t S;
     uint32_t m[OZTT_MAXS], y[OZTT_MAXS], magic[OZTT_MAXS], shift[OZTT_MAXS];
