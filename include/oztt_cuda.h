@@ -470,6 +470,49 @@ typedef struct oztt_linear_grad {
 } oztt_linear_grad;
 int oztt_linear_backward(int device_id, const oztt_linear_grad* args, void* stream, char* err, size_t errlen);
 
+/* ---- AdamW over many tensors -----------------------------------------------------------------------
+ * No counterpart in the reference. With g = grad * scale, in 32 bits:
+ *   m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2,
+ *   p' = p (1 - lr weight_decay) - lr / (1 - beta1^step) m' / (sqrt(v' / (1 - beta2^step)) + eps).
+ * The moments of all tensors lie in flat buffers: tensor i starts at element 256 * (the sum over the tensors
+ * before it of ceil(count / 256)), and the elements up to its last block's end are the library's to write. Zeroed
+ * buffers are zero moments. With 32 bits m and v are float; with 8 they are bytes, with one exponent byte E for
+ * each 256 in m_exp and v_exp: a code c > 0 stands for the float whose bits are (8 E + c) << 20 (m: c the low 7
+ * bits, the sign above them), 0 for zero. Codes are rounded stochastically, by random bits hashed from the element's
+ * position in the flat buffers and seed (give each step another), from the 32-bit m' and v' that the step uses; a
+ * v' > 0 is never stored as zero. A gradient that is not finite makes its parameter so, and the 8-bit moments of its
+ * block of 256 elements meaningless. Asynchronous on `stream`; one launch for up to 600 tensors. */
+enum { OZTT_TYPE_BF16 = 0, OZTT_TYPE_FP16 = 1, OZTT_TYPE_FP32 = 2 };
+#define OZTT_ADAMW_BLOCK 256
+
+typedef struct oztt_adamw_tensor {
+    void* param;
+    const void* grad;  /* NULL: the tensor, its moments included, stays as it is */
+    float* master;     /* optional: the step is taken on this copy, and param receives its rounding */
+    uint64_t count;    /* contiguous elements */
+    int32_t param_type, grad_type; /* OZTT_TYPE_* */
+} oztt_adamw_tensor;
+
+typedef struct oztt_adamw_moments {
+    int32_t bits; /* 8 or 32 */
+    void *m, *v;  /* 16-byte aligned */
+    uint8_t *m_exp, *v_exp; /* with 8 bits */
+} oztt_adamw_moments;
+
+typedef struct oztt_adamw_hyper {
+    double lr, beta1, beta2, eps, weight_decay;
+    uint64_t step; /* from 1 */
+    const float* grad_scale; /* optional, on the device: the factor of every gradient (a clipping coefficient) */
+    uint32_t seed;
+} oztt_adamw_hyper;
+
+int oztt_adamw_step(int device_id, const oztt_adamw_tensor* tensors, uint64_t count,
+                    const oztt_adamw_moments* moments, const oztt_adamw_hyper* hyper, void* stream, char* err,
+                    size_t errlen);
+/* The values of 8-bit moments, `blocks` blocks of 256 elements, as BF16, which holds each exactly. */
+int oztt_adamw_values(int device_id, const oztt_adamw_moments* moments, uint64_t blocks, uint16_t* m_out,
+                      uint16_t* v_out, void* stream, char* err, size_t errlen);
+
 /* Number of SMs and compute capability of a device (0 on success). */
 int oztt_device_info(int device_id, int32_t* sm_count, int32_t* cc_major, int32_t* cc_minor);
 

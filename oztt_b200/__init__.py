@@ -13,7 +13,7 @@ throws ``std::invalid_argument``, ``RuntimeError`` for ``std::runtime_error``, `
 expose the backend seam and the individual kernels for tests and benchmarks.
 
 ``linear`` and ``linear_backward`` (``layers.py``, on CUDA tensors of torch) are the 16-bit product of a
-network layer with its epilogue, and its gradients.
+network layer with its epilogue, and its gradients; ``AdamW`` (``optim.py``) steps many tensors at once.
 
 There is no CPU fallback: every compute call goes to the CUDA kernels, and importing the module
 fails if the library has not been built.
@@ -32,6 +32,7 @@ __all__ = [
     "Scheme", "Format", "Reconstruction", "Options", "DeviceOptions", "Info", "Context",
     "is_available", "format_name", "IIPlan", "ii_int8_plan", "ii_int8_run", "ii_int8_run_device",
     "lib", "library_path", "linear", "linear_backward",
+    "AdamW",
 ]
 
 _HERE = Path(__file__).resolve().parent
@@ -207,6 +208,8 @@ _SIGNATURES = {
     "oztt_resident_gemm": [_P, _P, _P, _I32, ctypes.POINTER(_COptions), ctypes.POINTER(_CInfo), _ERR, _SZ],
     "oztt_linear_forward": [ctypes.c_int, _P, _P, _ERR, _SZ],
     "oztt_linear_backward": [ctypes.c_int, _P, _P, _ERR, _SZ],
+    "oztt_adamw_step": [ctypes.c_int, _P, _U64, _P, _P, _P, _ERR, _SZ],
+    "oztt_adamw_values": [ctypes.c_int, _P, _U64, _P, _P, _P, _ERR, _SZ],
     "oztt_set_option": [_I32, _I32, _ERR, _SZ],
     "oztt_get_option": [_I32, ctypes.POINTER(_I32)],
     "oztt_is_available": [_I32],
@@ -252,7 +255,7 @@ def _lib() -> ctypes.CDLL:
 
 
 # What lives in modules that need torch, imported on first use.
-_TORCH_NAMES = {"linear": "layers", "linear_backward": "layers"}
+_TORCH_NAMES = {"linear": "layers", "linear_backward": "layers", "AdamW": "optim"}
 
 
 def __getattr__(name: str):

@@ -16,13 +16,13 @@
 // the residual are applied to the 32-bit sum, and each output is rounded once. dz is rounded once to the
 // operands' type, since the tensor core takes it so; db is summed from dz before that rounding.
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 #include <cstdint>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "device_scope.cuh"
 #include "runtime.cuh"
 #include "tensor_core.cuh"
 
@@ -548,28 +548,6 @@ static void check_view(const oztt_view& v, bool needed, const char* what) {
     if (reinterpret_cast<uintptr_t>(v.data) & 1) throw Error(OZTT_EINVAL, std::string(what) + " must be 2-byte aligned");
     if (v.row_stride < 0 || v.col_stride < 0) throw Error(OZTT_EINVAL, std::string(what) + ": strides must not be negative");
 }
-
-// Makes `device` current for one call.
-struct DeviceScope {
-    int before = 0;
-    bool changed = false;
-    explicit DeviceScope(int device) {
-        if (device < 0) throw Error(OZTT_EINVAL, "device_id must be nonnegative");
-        OZTT_CUDA(cudaGetDevice(&before));
-        if (before != device) {
-            OZTT_CUDA(cudaSetDevice(device));
-            changed = true;
-        }
-        static std::atomic<uint64_t> opened{0};
-        if (device < 64 && !(opened.load() >> device & 1)) {
-            open_device(device);
-            opened.fetch_or(1ull << device);
-        }
-    }
-    ~DeviceScope() {
-        if (changed) cudaSetDevice(before);
-    }
-};
 
 static void forward(int device, const oztt_linear& a, cudaStream_t st) {
     const int half = half_of(a.format, "linear");

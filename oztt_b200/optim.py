@@ -1,0 +1,181 @@
+"""AdamW over many CUDA tensors of torch in one launch, with moments in 32 bits or in 8 (oztt_adamw_step of the
+C ABI). No counterpart in the reference."""
+
+from __future__ import annotations
+
+import struct
+from operator import attrgetter
+
+import numpy as np
+import torch
+
+from . import OK, _errbuf, _lib, _raise
+
+__all__ = ["AdamW"]
+
+BLOCK = 256  # OZTT_ADAMW_BLOCK: elements of the moments that share an exponent
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # OZTT_TYPE_*
+
+# oztt_adamw_tensor, oztt_adamw_moments and oztt_adamw_hyper
+_TENSOR = np.dtype([("param", np.uint64), ("grad", np.uint64), ("master", np.uint64), ("count", np.uint64),
+                    ("param_type", np.int32), ("grad_type", np.int32)])
+_MOMENTS = struct.Struct("=i4x4Q")
+_HYPER = struct.Struct("=5dQQI4x")
+
+_dtype, _device = attrgetter("dtype"), attrgetter("device")
+
+
+class AdamW:
+    """The AdamW optimiser of a list of tensors (Adam with decoupled weight decay), one launch a step.
+
+        m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+
+    params: contiguous BF16, FP16 or FP32 tensors of one CUDA device that do not overlap; they are updated in place.
+    state_bits: 32, or 8 for moments of one byte an element, blocks of 256 elements sharing an exponent, rounded
+    stochastically (by `seed` and the step's number, so that a run can be repeated).
+    masters: FP32 copies of the parameters that the steps are taken on (a list as long as params, with None for
+    those without), or True to make them; without, the step is taken on the parameter's own value and rounded to
+    its type to nearest, which loses steps smaller than half its spacing.
+    """
+
+    def __init__(self, params, *, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 0.01, state_bits: int = 32, masters=None, seed: int = 0):
+        params = list(params)
+        if not params:
+            raise ValueError("AdamW: no parameters")
+        if state_bits not in (8, 32):
+            raise ValueError("AdamW: state_bits must be 8 or 32")
+        device = params[0].device
+        if device.type != "cuda":
+            raise ValueError("AdamW: the parameters must be on a CUDA device")
+        if masters is True:
+            masters = [None if p.dtype == torch.float32 else p.detach().float() for p in params]
+        masters = [None] * len(params) if masters is None or masters is False else list(masters)
+        if len(masters) != len(params):
+            raise ValueError("AdamW: masters must be as many as params")
+        spans = []
+        for i, (p, w) in enumerate(zip(params, masters)):
+            if p.dtype not in _TYPES or p.device != device or not p.is_contiguous():
+                raise ValueError(f"AdamW: parameter {i} must be a contiguous BF16, FP16 or FP32 tensor on {device}")
+            spans.append((p.data_ptr(), p.numel() * p.element_size()))
+            if w is not None:
+                if w.dtype != torch.float32 or w.device != device or not w.is_contiguous() or w.shape != p.shape:
+                    raise ValueError(f"AdamW: master {i} must be a contiguous FP32 tensor like its parameter")
+                spans.append((w.data_ptr(), w.numel() * 4))
+        end = 0
+        for at, size in sorted(s for s in spans if s[1]):
+            if at < end:
+                raise ValueError("AdamW: parameters overlap")
+            end = at + size
+        self.params, self.masters, self.state_bits, self.device, self.seed = params, masters, state_bits, device, seed
+        self.lr, self.betas, self.eps, self.weight_decay = lr, tuple(betas), eps, weight_decay
+        self.t = 0
+        self._counts = [p.numel() for p in params]
+        blocks = [-(-n // BLOCK) for n in self._counts]
+        self.blocks = sum(blocks)
+        # where each tensor's part of the flat moments starts
+        self.offsets = [BLOCK * (sum_ - b) for b, sum_ in zip(blocks, np.cumsum(blocks).tolist())]
+        kind = torch.uint8 if state_bits == 8 else torch.float32
+        zeros = lambda n, dtype: torch.zeros(n, dtype=dtype, device=device)  # noqa: E731
+        self.m, self.v = zeros(self.blocks * BLOCK, kind), zeros(self.blocks * BLOCK, kind)
+        self.m_exp = self.v_exp = None
+        if state_bits == 8:
+            self.m_exp, self.v_exp = zeros(self.blocks, kind), zeros(self.blocks, kind)
+        self._table = np.zeros(len(params), _TENSOR)
+        self._table["param"] = [p.data_ptr() for p in params]
+        self._table["master"] = [0 if w is None else w.data_ptr() for w in masters]
+        self._table["count"] = self._counts
+        self._table["param_type"] = [_TYPES[p.dtype] for p in params]
+        self._grown = [p for p in params if p.requires_grad]
+        self._err = _errbuf()
+
+    def _moments(self) -> bytes:
+        exps = (self.m_exp.data_ptr(), self.v_exp.data_ptr()) if self.state_bits == 8 else (0, 0)
+        return _MOMENTS.pack(self.state_bits, self.m.data_ptr(), self.v.data_ptr(), *exps)
+
+    def _call(self, name: str, *args) -> None:
+        rc = getattr(_lib(), name)(self.device.index, *args, torch._C._cuda_getCurrentRawStream(self.device.index),
+                                   self._err, len(self._err))
+        if rc != OK:
+            _raise(rc, self._err.value)
+
+    def step(self, grads=None, *, grad_scale: torch.Tensor | None = None, lr: float | None = None,
+             seed: int | None = None) -> None:
+        """One step on the current stream, without waiting for it. grads: a gradient for each parameter (contiguous,
+        of the parameter's size, BF16, FP16 or FP32), None for one that stays as it is; by default the parameters'
+        .grad. grad_scale: one FP32 number on the device that every gradient is multiplied by (a clipping
+        coefficient). lr: this step's learning rate. seed: of this step's rounding, by default from the optimiser's
+        seed and the step's number. The step's number and rates are numbers of the launch: a CUDA graph of it
+        repeats the same step."""
+        if grads is None:
+            grads = [p.grad for p in self.params]
+        if len(grads) != len(self.params):
+            raise ValueError("AdamW: grads must be as many as params")
+        table = self._table
+        counts, live = self._counts, grads
+        if any(g is None for g in grads):
+            counts = [n for n, g in zip(counts, grads) if g is not None]
+            live = [g for g in grads if g is not None]
+        if live:
+            kinds = set(map(_dtype, live))
+            if not kinds <= _TYPES.keys():
+                raise ValueError("AdamW: gradients must be BF16, FP16 or FP32")
+            if set(map(_device, live)) != {self.device}:
+                raise ValueError(f"AdamW: gradients must be on {self.device}")
+            if list(map(torch.Tensor.numel, live)) != counts:
+                raise ValueError("AdamW: a gradient's size is not its parameter's")
+            if not all(map(torch.Tensor.is_contiguous, live)):
+                raise ValueError("AdamW: gradients must be contiguous")
+            if live is grads:
+                table["grad"] = list(map(torch.Tensor.data_ptr, grads))
+                table["grad_type"] = _TYPES[next(iter(kinds))] if len(kinds) == 1 else [_TYPES[g.dtype] for g in grads]
+            else:
+                table["grad"] = [0 if g is None else g.data_ptr() for g in grads]
+                table["grad_type"] = [0 if g is None else _TYPES[g.dtype] for g in grads]
+        else:
+            table["grad"] = 0
+        if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.device != self.device
+                                       or grad_scale.numel() != 1):
+            raise ValueError(f"AdamW: grad_scale must be one FP32 number on {self.device}")
+        t = self.t + 1
+        if seed is None:
+            seed = self.seed + 0x632BE5AB * t
+        hyper = _HYPER.pack(self.lr if lr is None else lr, *self.betas, self.eps, self.weight_decay, t,
+                            0 if grad_scale is None else grad_scale.data_ptr(), seed & 0xFFFFFFFF)
+        self._call("oztt_adamw_step", table.ctypes.data, len(self.params), self._moments(), hyper)
+        self.t = t
+        if self._grown:  # saved for a backward pass that has not run, they are no longer what was saved
+            torch.autograd.graph.increment_version(self._grown)
+
+    def moments(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """The flat moments (m, v), tensor i's from offsets[i] on: the FP32 buffers themselves with 32 bits, new
+        BF16 tensors with 8, which hold the values of the codes exactly."""
+        if self.state_bits == 32:
+            return self.m, self.v
+        m, v = (torch.empty(self.blocks * BLOCK, dtype=torch.bfloat16, device=self.device) for _ in range(2))
+        self._call("oztt_adamw_values", self._moments(), self.blocks, m.data_ptr(), v.data_ptr())
+        return m, v
+
+    def state_dict(self) -> dict:
+        """What load_state_dict needs to go on from here: the number of steps, the moments as they are kept, and the
+        masters. The tensors are the optimiser's own."""
+        d = {"t": self.t, "state_bits": self.state_bits, "seed": self.seed, "m": self.m, "v": self.v,
+             "masters": self.masters}
+        if self.state_bits == 8:
+            d["m_exp"], d["v_exp"] = self.m_exp, self.v_exp
+        return d
+
+    def load_state_dict(self, d: dict) -> None:
+        """Copies a state_dict of an optimiser of like tensors and bits."""
+        names = ["m", "v"] + (["m_exp", "v_exp"] if self.state_bits == 8 else [])
+        if d.get("state_bits") != self.state_bits or any(d[n].shape != getattr(self, n).shape for n in names):
+            raise ValueError("AdamW: the state is of other tensors or bits")
+        if [w is None for w in d["masters"]] != [w is None for w in self.masters]:
+            raise ValueError("AdamW: the state has other masters")
+        for n in names:
+            getattr(self, n).copy_(d[n])
+        for w, s in zip(self.masters, d["masters"]):
+            if w is not None:
+                w.copy_(s)
+        self.t, self.seed = int(d["t"]), int(d["seed"])
