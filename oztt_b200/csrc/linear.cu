@@ -51,8 +51,8 @@ struct Epilogue {
     View out, pre, res;                  // pre and res may be null
     const void* bias;                    // may be null
     int64_t bias_stride;
-    int32_t act, half;                   // OZTT_ACT_*; 1: FP16, 0: BF16
-    int32_t vec;                         // 4 columns at a time: unit column strides and 8-byte aligned rows
+    int32_t act;                         // OZTT_ACT_*
+    int32_t vec;                         // columns that one access may take: 1, 4 or 8
 };
 
 // ---- activations in 32 bits ----------------------------------------------------------------------
@@ -60,15 +60,31 @@ __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f
 constexpr float kTanhScale = 0.7978845608028654f;  // sqrt(2/pi)
 constexpr float kTanhCube = 0.044715f;
 
+// The normal distribution's cumulative function, and e = exp(-z^2 / 2) on the way: the rational approximation
+// 7.1.26 of Abramowitz and Stegun's Handbook of Mathematical Functions (erfc x = t (a1 + t (a2 + ...)) exp(-x^2),
+// t = 1 / (1 + p x), off by at most 1.5e-7, which the 16-bit results do not show). It has no branch and, formed
+// for the lower tail, no cancellation.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    float q = fmaf(1.061405429f, t, -1.453152027f);
+    q = fmaf(q, t, 1.421413741f);
+    q = fmaf(q, t, -0.284496736f);
+    q = fmaf(q, t, 0.254829592f);
+    e = __expf(-x * x);
+    const float tail = 0.5f * q * t * e;
+    return z < 0.0f ? tail : 1.0f - tail;
+}
+
 // gelu_tanh is z (1 + tanh u) / 2 = z sigmoid(2u): no cancellation in the lower tail.
 __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {
         case OZTT_ACT_RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
-        case OZTT_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-        case OZTT_ACT_GELU_TANH: {
-            const float u = kTanhScale * (z + kTanhCube * z * z * z);
-            return z * sigmoid(2.0f * u);
+        case OZTT_ACT_GELU: {
+            float e;
+            return z * normal_cdf(z, e);
         }
+        case OZTT_ACT_GELU_TANH: return z * sigmoid(2.0f * kTanhScale * z * fmaf(kTanhCube * z, z, 1.0f));
         case OZTT_ACT_SILU: return z * sigmoid(z);
         default: return z;
     }
@@ -76,11 +92,14 @@ __device__ __forceinline__ float activate(float z, int act) {
 __device__ __forceinline__ float slope(float z, int act) {
     switch (act) {
         case OZTT_ACT_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-        case OZTT_ACT_GELU:
-            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.3989422804014327f;
+        case OZTT_ACT_GELU: {
+            float e;
+            const float c = normal_cdf(z, e);
+            return fmaf(z * 0.3989422804014327f, e, c);
+        }
         case OZTT_ACT_GELU_TANH: {
-            const float s = sigmoid(2.0f * kTanhScale * (z + kTanhCube * z * z * z));
-            return s + 2.0f * z * s * (1.0f - s) * kTanhScale * (1.0f + 3.0f * kTanhCube * z * z);
+            const float zz = z * z, s = sigmoid(2.0f * kTanhScale * z * fmaf(kTanhCube, zz, 1.0f));
+            return s + 2.0f * z * s * (1.0f - s) * kTanhScale * fmaf(3.0f * kTanhCube, zz, 1.0f);
         }
         case OZTT_ACT_SILU: {
             const float s = sigmoid(z);
@@ -90,11 +109,50 @@ __device__ __forceinline__ float slope(float z, int act) {
     }
 }
 
-__device__ __forceinline__ float to_f32(uint16_t v, int half) {
-    return half ? __half2float(__ushort_as_half(v)) : __uint_as_float((uint32_t)v << 16);
+// FP16 (HALF) or BF16 values by their bits; a pair has its first value in the low half.
+template <bool HALF>
+__device__ __forceinline__ float to_f32(uint32_t v) {
+    return HALF ? __half2float(__ushort_as_half((unsigned short)v)) : __uint_as_float(v << 16);
 }
-__device__ __forceinline__ uint16_t from_f32(float v, int half) {
-    return half ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+template <bool HALF>
+__device__ __forceinline__ uint16_t from_f32(float v) {
+    return HALF ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+template <bool HALF>
+__device__ __forceinline__ void unpack(uint32_t w, float& lo, float& hi) {
+    if (HALF) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        lo = f.x, hi = f.y;
+    } else {
+        lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xFFFF0000u);
+    }
+}
+template <bool HALF>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t w;
+    if (HALF)
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    else
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+}
+
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// 16-bit values w.. by one access of 8 or 16 bytes.
+__device__ __forceinline__ void load_words(const uint16_t* p, uint32_t (&w)[2]) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+}
+__device__ __forceinline__ void load_words(const uint16_t* p, uint32_t (&w)[4]) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+}
+__device__ __forceinline__ void store_words(uint16_t* p, const uint32_t (&w)[2]) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ void store_words(uint16_t* p, const uint32_t (&w)[4]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ---- the tile product ----------------------------------------------------------------------------
@@ -140,6 +198,12 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
     return v;
 }
 
+__device__ __forceinline__ float ld_cluster_f1(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
 // One operand's 64-element block of the reduction into shared memory: one box of `rows` rows when K-major, one
 // for every 64 rows when MN-major. Coordinates outside the matrix read as zero.
 __device__ __forceinline__ void load_operand(const CUtensorMap* map, uint32_t dst, uint64_t* bar, int32_t row,
@@ -152,43 +216,97 @@ __device__ __forceinline__ void load_operand(const CUtensorMap* map, uint32_t ds
     }
 }
 
-// Bias, activation, residual and the stores of four neighbouring columns j .. j+3 of row i.
-__device__ __forceinline__ void finish4(const Epilogue& e, uint64_t i, uint64_t j, float4 acc, const float (&bias)[4]) {
-    float z[4] = {acc.x + bias[0], acc.y + bias[1], acc.z + bias[2], acc.w + bias[3]};
-    const bool whole = e.vec && j + 3 < e.cols;
-    uint16_t* out = reinterpret_cast<uint16_t*>(e.out.p) + (int64_t)i * e.out.rs + (int64_t)j * e.out.cs;
-    uint16_t* pre = reinterpret_cast<uint16_t*>(e.pre.p) + (int64_t)i * e.pre.rs + (int64_t)j * e.pre.cs;
-    const uint16_t* res = reinterpret_cast<const uint16_t*>(e.res.p) + (int64_t)i * e.res.rs + (int64_t)j * e.res.cs;
-    if (whole) {
-        float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (e.res.p) {
-            const ushort4 v = *reinterpret_cast<const ushort4*>(res);
-            r[0] = to_f32(v.x, e.half), r[1] = to_f32(v.y, e.half), r[2] = to_f32(v.z, e.half), r[3] = to_f32(v.w, e.half);
-        }
-        if (e.pre.p)
-            *reinterpret_cast<ushort4*>(pre) = make_ushort4(from_f32(z[0], e.half), from_f32(z[1], e.half),
-                                                            from_f32(z[2], e.half), from_f32(z[3], e.half));
+// The sums of N values through the activation: the choice is made once for the N.
+template <int N>
+__device__ __forceinline__ void activate_all(float (&z)[N], int act) {
+    switch (act) {
+#define OZTT_CASE(A) \
+    case A:          \
+        _Pragma("unroll") for (int q = 0; q < N; ++q) z[q] = activate(z[q], A); \
+        break;
+        OZTT_CASE(OZTT_ACT_RELU)
+        OZTT_CASE(OZTT_ACT_GELU)
+        OZTT_CASE(OZTT_ACT_GELU_TANH)
+        OZTT_CASE(OZTT_ACT_SILU)
+#undef OZTT_CASE
+        default: break;
+    }
+}
+
+__device__ __forceinline__ void slope_all(float (&z)[8], int act) {
+    switch (act) {
+#define OZTT_CASE(A) \
+    case A:          \
+        _Pragma("unroll") for (int q = 0; q < 8; ++q) z[q] = slope(z[q], A); \
+        break;
+        OZTT_CASE(OZTT_ACT_RELU)
+        OZTT_CASE(OZTT_ACT_GELU)
+        OZTT_CASE(OZTT_ACT_GELU_TANH)
+        OZTT_CASE(OZTT_ACT_SILU)
+#undef OZTT_CASE
+        default: break;
+    }
+}
+
+__device__ __forceinline__ uint16_t* element(const View& v, uint64_t i, uint64_t j) {
+    return reinterpret_cast<uint16_t*>(v.p) + (int64_t)i * v.rs + (int64_t)j * v.cs;
+}
+
+// Activation, residual and the stores of N neighbouring columns, their bias added: every one of them exists, and the
+// views take accesses of N values. out, pre (or null): where they go; r: the residual's words, if has_res.
+template <bool HALF, int N>
+__device__ __forceinline__ void finish_vector(uint16_t* out, uint16_t* pre, bool has_res, int act, float (&z)[N],
+                                              const uint32_t (&r)[N / 2]) {
+    uint32_t w[N / 2];
+    if (pre) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) z[q] = activate(z[q], e.act) + r[q];
-        *reinterpret_cast<ushort4*>(out) = make_ushort4(from_f32(z[0], e.half), from_f32(z[1], e.half),
-                                                        from_f32(z[2], e.half), from_f32(z[3], e.half));
-    } else {
+        for (int q = 0; q < N / 2; ++q) w[q] = pack<HALF>(z[2 * q], z[2 * q + 1]);
+        store_words(pre, w);
+    }
+    activate_all<N>(z, act);
+    if (has_res) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if (j + q >= e.cols) continue;
-            if (e.pre.p) pre[q * e.pre.cs] = from_f32(z[q], e.half);
-            float y = activate(z[q], e.act);
-            if (e.res.p) y += to_f32(res[q * e.res.cs], e.half);
-            out[q * e.out.cs] = from_f32(y, e.half);
+        for (int q = 0; q < N / 2; ++q) {
+            float lo, hi;
+            unpack<HALF>(r[q], lo, hi);
+            z[2 * q] += lo, z[2 * q + 1] += hi;
         }
     }
+#pragma unroll
+    for (int q = 0; q < N / 2; ++q) w[q] = pack<HALF>(z[2 * q], z[2 * q + 1]);
+    store_words(out, w);
+}
+// The same for any N values, (di, dj) apart, of which those inside the output are finished, by accesses of one value.
+template <bool HALF, int N>
+__device__ __forceinline__ void finish_scattered(const Epilogue& e, uint64_t i, uint64_t j, uint32_t di, uint32_t dj,
+                                                 float (&z)[N]) {
+    uint16_t r[N];
+    bool in[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        in[q] = i + q * di < e.rows && j + q * dj < e.cols;
+        r[q] = e.res.p && in[q] ? *element(e.res, i + q * di, j + q * dj) : 0;
+    }
+    if (e.pre.p) {
+#pragma unroll
+        for (int q = 0; q < N; ++q)
+            if (in[q]) *element(e.pre, i + q * di, j + q * dj) = from_f32<HALF>(z[q]);
+    }
+    activate_all<N>(z, e.act);
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+        if (in[q]) *element(e.out, i + q * di, j + q * dj) = from_f32<HALF>(e.res.p ? z[q] + to_f32<HALF>(r[q]) : z[q]);
+}
+template <bool HALF>
+__device__ __forceinline__ float bias_at(const Epilogue& e, uint64_t j) {
+    return e.bias && j < e.cols ? to_f32<HALF>(reinterpret_cast<const uint16_t*>(e.bias)[(int64_t)j * e.bias_stride]) : 0.0f;
 }
 
 // One tile of 128 output columns by BQ output rows per cluster; the CTAs of a cluster share the reduction: each
 // sums its stretch of it in tensor memory and lays the 32-bit sums down in its own shared memory (where the
 // operand stages were), then each finishes its share of the rows, adding the stretches in the cluster's order
 // through distributed shared memory, so the result does not depend on timing.
-template <int BQ, int STAGES, int CTAS>
+template <bool HALF, int BQ, int STAGES, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS)
     product_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ, const Product pr,
                    const Epilogue e, int* err) {
@@ -306,30 +424,43 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     __syncthreads();
     if (split > 1) cluster_sync();
 
-    const uint64_t j = (uint64_t)tp * BP + lane * 4;
-    if (j < e.cols) {
-        float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (e.bias) {
-            const uint16_t* b = reinterpret_cast<const uint16_t*>(e.bias);
+    // a lane finishes 4 neighbouring columns where the views allow it, else 4 columns 32 apart
+    const uint64_t j0 = (uint64_t)tp * BP;
+    const bool vec = e.vec >= 4 && j0 + BP <= e.cols;
+    uint64_t col[4];
+    float bias[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (j + q < e.cols) bias[q] = to_f32(b[(int64_t)(j + q) * e.bias_stride], e.half);
-        }
-        const uint32_t r0 = BQ * rank / split, r1 = BQ * (rank + 1) / split;
-        const uint32_t mine = smem_u32(smem) + lane * 16;
-        for (uint32_t r = r0 + warp; r < r1; r += THREADS / 32) {
-            const uint64_t i = (uint64_t)tq * BQ + r;
-            if (i >= e.rows) break;
+    for (int q = 0; q < 4; ++q) {
+        col[q] = j0 + (vec ? lane * 4 + q : lane + 32 * q);
+        bias[q] = bias_at<HALF>(e, col[q]);
+    }
+    const uint32_t r0 = BQ * rank / split, r1 = BQ * (rank + 1) / split;
+    for (uint32_t r = r0 + warp; r < r1; r += THREADS / 32) {
+        const uint64_t i = (uint64_t)tq * BQ + r;
+        if (i >= e.rows) break;
+        float z[4] = {bias[0], bias[1], bias[2], bias[3]};
+        const uint32_t row = smem_u32(smem) + r * (BP * 4);
+        if (vec) {
+            uint32_t res[2] = {0, 0};
+            if (e.res.p) load_words(element(e.res, i, col[0]), res);
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (split == 1) {
-                acc = *reinterpret_cast<const float4*>(smem + r * (BP * 4) + lane * 16);
-            } else {
-                for (uint32_t c = 0; c < split; ++c) {
-                    const float4 v = ld_cluster_f4(map_to(mine + r * (BP * 4), c));
-                    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-                }
+            for (uint32_t c = 0; c < split; ++c) {
+                const float4 v = ld_cluster_f4(map_to(row + lane * 16, c));
+                acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
             }
-            finish4(e, i, j, acc, bias);
+            z[0] += acc.x, z[1] += acc.y, z[2] += acc.z, z[3] += acc.w;
+            finish_vector<HALF, 4>(element(e.out, i, col[0]), e.pre.p ? element(e.pre, i, col[0]) : nullptr, e.res.p, e.act,
+                                   z, res);
+        } else {
+            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t c = 0; c < split; ++c) {
+                const uint32_t at = map_to(row + lane * 4, c);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[q] += ld_cluster_f1(at + 128 * q);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) z[q] += acc[q];
+            finish_scattered<HALF, 4>(e, i, col[0], 0, 32, z);
         }
     }
     __syncthreads();
@@ -337,6 +468,265 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS)
+                     : "memory");
+    }
+}
+
+// ---- the pair product: large outputs -----------------------------------------------------------
+// The same product on CTA pairs (cta_group::2): a tile of 256 output columns by BQ output rows, each CTA of the
+// pair holding 128 of the columns and half of Q's rows, so that shared memory feeds the tensor cores with the
+// fewest bytes. Persistent: the pairs walk over the tiles, the sums of one tile are finished from one half of
+// tensor memory while the next tile accumulates in the other. Sixteen warps finish them (the latencies of the path
+// from tensor memory to the stores need so many), each 32 columns of a quarter of the rows: 8 rows at a time go
+// through a patch of shared memory of the warp's own, from which a lane takes 8 neighbouring columns of a row, so
+// that bias, activation, residual and stores run on 16-byte accesses.
+constexpr uint32_t PAIR_STAGES_BYTES = 196608;
+constexpr uint32_t FINISHERS = 16;
+constexpr uint32_t PAIR_THREADS = (2 + FINISHERS) * 32;  // warp 0 loads, warp 1 issues, the others finish
+constexpr uint32_t PATCH_ROWS = 8, PATCH_LD = 36;  // padded: neither its rows nor its columns share banks
+constexpr uint32_t PATCH_BYTES = PATCH_ROWS * PATCH_LD * 4;
+constexpr uint32_t GROUP_Q = 8;         // rows of tiles that the running pairs share in L2
+constexpr uint64_t PEER_DRAIN_NS = 5000000ull;
+
+__device__ __forceinline__ void tma_load_2d_pair(const CUtensorMap* map, uint32_t dst, uint32_t bar_cluster, int32_t c0,
+                                                 int32_t c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+        "%4}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(c0), "r"(c1)
+        : "memory");
+}
+__device__ __forceinline__ void load_operand_pair(const CUtensorMap* map, uint32_t dst, uint32_t bar_cluster,
+                                                  int32_t row, int32_t k, uint32_t rows, uint32_t mn) {
+    if (mn) {
+        for (uint32_t b = 0; b < rows / MN_BOX; ++b)
+            tma_load_2d_pair(map, dst + b * MN_BOX_BYTES, bar_cluster, row + (int32_t)(b * MN_BOX), k);
+    } else {
+        tma_load_2d_pair(map, dst, bar_cluster, k, row);
+    }
+}
+__device__ __forceinline__ void umma_16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Tile number -> tile column tp, tile row tq: groups of GROUP_Q tile rows, each walked column by column.
+__device__ __forceinline__ void tile_at(uint32_t tile, uint32_t tiles_p, uint32_t tiles_q, uint32_t& tp, uint32_t& tq) {
+    const uint32_t span = GROUP_Q * tiles_p, g = tile / span, first = g * GROUP_Q;
+    const uint32_t size = min(tiles_q - first, GROUP_Q), r = tile - g * span;
+    tq = first + r % size;
+    tp = r / size;
+}
+
+template <bool HALF, int BQ>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+    pair_product_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
+                        const Product pr, const uint32_t tiles_q, const Epilogue e, int* err) {
+    constexpr uint32_t HALF_Q = BQ / 2;
+    constexpr uint32_t STAGE_BYTES = P_BYTES + HALF_Q * BK * 2;
+    constexpr uint32_t STAGES = PAIR_STAGES_BYTES / STAGE_BYTES;
+    constexpr uint32_t TMEM_COLS = 2 * BQ;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* patches = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES + FINISHERS * PATCH_BYTES);
+    uint64_t* empty_bar = full_bar + STAGES;
+    uint64_t* tfull_bar = empty_bar + STAGES;
+    uint64_t* tempty_bar = tfull_bar + 2;
+    uint64_t* drain_bar = tempty_bar + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const uint32_t first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
+    const uint32_t num_tiles = pr.tiles_p * tiles_q;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < STAGES; ++s) {
+            mbar_init(full_bar + s, 1);
+            mbar_init(empty_bar + s, 1);
+        }
+        for (uint32_t a = 0; a < 2; ++a) {
+            mbar_init(tfull_bar + a, 1);
+            mbar_init(tempty_bar + a, 2 * FINISHERS);  // the finishing warps of both CTAs
+        }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // the peer's barriers are initialised before anything is signalled across the pair
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0, filled = 0, last_phase = 0;
+            bool ok = true, issued = false;
+            for (uint32_t tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
+                uint32_t tp, tq;
+                tile_at(tile, pr.tiles_p, tiles_q, tp, tq);
+                for (uint32_t kb = 0; kb < pr.num_kb; ++kb) {
+                    if (!mbar_wait(empty_bar + stage, phase ^ 1u, abort_flag, err, ERR_WAIT_PRODUCER)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) mbar_expect_tx(full_bar + stage, 2 * STAGE_BYTES);
+                    const uint32_t full_leader = map_to(smem_u32(full_bar + stage), 0);
+                    const uint32_t sp = smem_u32(smem + stage * STAGE_BYTES);
+                    load_operand_pair(&tmP, sp, full_leader, (int32_t)(tp * 2 * BP + rank * BP), (int32_t)(kb * BK), BP,
+                                      pr.p_mn);
+                    load_operand_pair(&tmQ, sp + P_BYTES, full_leader, (int32_t)(tq * BQ + rank * HALF_Q),
+                                      (int32_t)(kb * BK), HALF_Q, pr.q_mn);
+                    issued = true;
+                    filled |= 1u << stage;
+                    last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (!ok) {  // let the loads this thread issued land before the CTA may exit
+                if (rank == 0) {
+                    for (uint32_t st = 0; st < STAGES; ++st)
+                        if (filled & (1u << st)) mbar_wait_drain(full_bar + st, (last_phase >> st) & 1u, 200000000ull);
+                } else if (issued) {  // the peer's loads complete on the leader's barriers: wait a fixed time
+                    const uint64_t t0 = global_timer_ns();
+                    while (global_timer_ns() - t0 < PEER_DRAIN_NS) {
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+            const uint32_t step_p = pr.p_mn ? UK * 128u : UK * 2u, step_q = pr.q_mn ? UK * 128u : UK * 2u;
+            bool ok = true;
+            for (uint32_t tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
+                if (!mbar_wait(tempty_bar + acc, acc_phase ^ 1u, abort_flag, err, ERR_WAIT_MMA_EMPTY)) break;
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + acc * BQ;
+                for (uint32_t kb = 0; kb < pr.num_kb; ++kb) {
+                    if (!mbar_wait(full_bar + stage, phase, abort_flag, err, ERR_WAIT_MMA_FULL)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sp = smem_u32(smem + stage * STAGE_BYTES), sq = sp + P_BYTES;
+#pragma unroll
+                    for (uint32_t k = 0; k < BK / UK; ++k)
+                        umma_16_pair(d_tmem, operand_desc(sp + k * step_p, pr.p_mn),
+                                     operand_desc(sq + k * step_q, pr.q_mn), pr.idesc, (kb | k) != 0u);
+                    const uint32_t eb = smem_u32(empty_bar + stage);
+                    umma_commit_pair(eb);
+                    umma_commit_pair(map_to(eb, 1));
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                const uint32_t tb = smem_u32(tfull_bar + acc);
+                umma_commit_pair(tb);
+                umma_commit_pair(map_to(tb, 1));
+                acc ^= 1u;
+                if (acc == 0) acc_phase ^= 1u;
+            }
+            // Every product this thread issued completes before the columns of either CTA are freed.
+            umma_commit_pair(smem_u32(drain_bar));
+            mbar_wait_drain(drain_bar, 0, 1000000000ull);
+        }
+    } else {
+        // 32 columns (a quarter of the CTA's) by a quarter of the tile's rows
+        constexpr uint32_t ROWS = BQ / (FINISHERS / 4);
+        const uint32_t quarter = warp & 3u, c0 = ((warp - 2) >> 2) * ROWS;
+        float* patch = patches + (warp - 2) * (PATCH_BYTES / 4);
+        const uint32_t prow = lane >> 2, pcol = (lane & 3u) * 8u;
+        uint32_t acc = 0, acc_phase = 0;
+        for (uint32_t tile = first_tile; tile < num_tiles; tile += tile_step) {
+            uint32_t tp, tq;
+            tile_at(tile, pr.tiles_p, tiles_q, tp, tq);
+            const uint64_t j0 = (uint64_t)tp * 2 * BP + rank * BP + quarter * 32u;
+            const uint64_t i0 = (uint64_t)tq * BQ + c0;
+            const bool vec = e.vec >= 8 && j0 + 32 <= e.cols;
+            float bias[8];
+            if (vec) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) bias[q] = bias_at<HALF>(e, j0 + pcol + q);
+            } else {
+                bias[0] = bias_at<HALF>(e, j0 + lane);
+            }
+            const uint32_t rows = j0 < e.cols && i0 < e.rows ? (uint32_t)min((uint64_t)ROWS, e.rows - i0) : 0;
+            // this lane's place in the first patch; the next is 8 rows further
+            uint16_t* out = element(e.out, i0 + prow, j0 + pcol);
+            uint16_t* pre = element(e.pre, i0 + prow, j0 + pcol);
+            const uint16_t* res = element(e.res, i0 + prow, j0 + pcol);
+            if (vec && e.res.p)
+                for (uint32_t c = prow; c < rows; c += PATCH_ROWS) prefetch_l2(res + (c - prow) * e.res.rs);
+            if (!mbar_wait(tfull_bar + acc, acc_phase, abort_flag, err, ERR_WAIT_EPILOGUE)) break;
+            tc_fence_after();
+            const uint32_t tbase = tmem_base + ((quarter * 32u) << 16) + acc * BQ + c0;
+            if (vec) {
+                const bool has_pre = e.pre.p, has_res = e.res.p;
+#pragma unroll 1
+                for (uint32_t c = 0; c < rows; c += PATCH_ROWS) {
+                    const bool mine = c + prow < rows;
+                    uint32_t r[4] = {}, v[8];
+                    if (has_res && mine) load_words(res, r);
+                    tmem_ld8(tbase + c, v);
+                    __syncwarp();  // the patch has been read
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) patch[q * PATCH_LD + lane] = __uint_as_float(v[q]);
+                    __syncwarp();
+                    const float4* p = reinterpret_cast<const float4*>(patch + prow * PATCH_LD + pcol);
+                    const float4 x = p[0], y = p[1];
+                    float z[8] = {x.x + bias[0], x.y + bias[1], x.z + bias[2], x.w + bias[3],
+                                  y.x + bias[4], y.y + bias[5], y.z + bias[6], y.w + bias[7]};
+                    if (mine) finish_vector<HALF, 8>(out, has_pre ? pre : nullptr, has_res, e.act, z, r);
+                    out += PATCH_ROWS * e.out.rs;
+                    pre += PATCH_ROWS * e.pre.rs;
+                    res += PATCH_ROWS * e.res.rs;
+                }
+            } else {
+#pragma unroll 1
+                for (uint32_t c = 0; c < rows; c += PATCH_ROWS) {
+                    uint32_t v[8];
+                    tmem_ld8(tbase + c, v);
+                    float z[8];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) z[q] = __uint_as_float(v[q]) + bias[0];
+                    finish_scattered<HALF, 8>(e, i0 + c, j0 + lane, 1, 0, z);
+                }
+            }
+            // the sums have been read: all that the arrival has to tell; a releasing one would also
+            // wait for the stores
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_remote_relaxed(map_to(smem_u32(tempty_bar + acc), 0));
+            acc ^= 1u;
+            if (acc == 0) acc_phase ^= 1u;
+        }
+    }
+    __syncthreads();
+    cluster_sync();  // no CTA frees its tensor memory or exits while the pair may still use it
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS)
                      : "memory");
     }
 }
@@ -364,32 +754,101 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint16_t* __restrict__ 
 }
 
 // dz = dy * act'(z) into dz (rows ld apart; may be null), and the sums of its columns over this block's rows in
-// 32 bits into partial[block row][n] (may be null). Block (x, y): 32 columns each of 8 warps by ROWS rows.
-constexpr uint32_t DZ_ROWS = 64;
-__global__ void __launch_bounds__(256) dz_kernel(View dy, View z, uint64_t m, uint64_t n, int act, int half,
-                                                 uint16_t* __restrict__ dz, uint64_t ld, float* __restrict__ partial) {
-    const uint64_t j = blockIdx.x * 256ull + threadIdx.x;
-    const uint64_t i0 = blockIdx.y * (uint64_t)DZ_ROWS, i1 = min(i0 + DZ_ROWS, m);
-    if (j >= n) return;
-    const uint16_t* gy = reinterpret_cast<const uint16_t*>(dy.p) + (int64_t)j * dy.cs;
-    const uint16_t* gz = reinterpret_cast<const uint16_t*>(z.p) + (int64_t)j * z.cs;
-    float sum = 0.0f;
-    for (uint64_t i = i0; i < i1; ++i) {
-        float v = to_f32(gy[(int64_t)i * dy.rs], half);
-        if (act != OZTT_ACT_NONE) v *= slope(to_f32(gz[(int64_t)i * z.rs], half), act);
-        sum += v;
-        if (dz) dz[i * ld + j] = from_f32(v, half);
+// 32 bits into partial[block row][n] (may be null), always in the same order. A block takes 256 columns by `span`
+// rows, a warp one row at a time, four rows' loads in flight. VEC: a lane takes 8 neighbouring columns by 16-byte
+// accesses, else 8 columns 32 apart.
+constexpr uint32_t DZ_COLS = 256, DZ_WARPS = 8, DZ_AHEAD = 4;
+template <bool HALF, bool VEC>
+__global__ void __launch_bounds__(DZ_WARPS * 32)
+    dz_kernel(View dy, View z, uint64_t m, uint64_t n, uint32_t span, int act, uint16_t* __restrict__ dz, uint64_t ld,
+              float* __restrict__ partial) {
+    __shared__ float sums[DZ_WARPS][DZ_COLS];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t j0 = blockIdx.x * (uint64_t)DZ_COLS + (VEC ? lane * 8 : lane);
+    const uint64_t i0 = blockIdx.y * (uint64_t)span, i1 = min(i0 + span, m);
+    const bool whole = VEC && j0 + 8 <= n;
+    constexpr uint32_t DJ = VEC ? 1 : 32;
+    float sum[8] = {};
+    for (uint64_t base = i0 + warp; base < i1; base += DZ_WARPS * DZ_AHEAD) {
+        uint32_t g[DZ_AHEAD][4], s[DZ_AHEAD][4];
+#pragma unroll
+        for (uint32_t a = 0; a < DZ_AHEAD; ++a) {
+            const uint64_t i = base + a * DZ_WARPS;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) g[a][q] = s[a][q] = 0;
+            if (i >= i1) continue;
+            if (whole) {
+                load_words(element(dy, i, j0), g[a]);
+                if (act != OZTT_ACT_NONE) load_words(element(z, i, j0), s[a]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const uint64_t j = j0 + q * DJ;
+                    if (j >= n) continue;
+                    g[a][q >> 1] |= (uint32_t)*element(dy, i, j) << (16 * (q & 1));
+                    if (act != OZTT_ACT_NONE) s[a][q >> 1] |= (uint32_t)*element(z, i, j) << (16 * (q & 1));
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t a = 0; a < DZ_AHEAD; ++a) {
+            const uint64_t i = base + a * DZ_WARPS;
+            if (i >= i1) continue;
+            float v[8];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) unpack<HALF>(g[a][q], v[2 * q], v[2 * q + 1]);
+            if (act != OZTT_ACT_NONE) {
+                float t[8];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) unpack<HALF>(s[a][q], t[2 * q], t[2 * q + 1]);
+                slope_all(t, act);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[q] *= t[q];
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) sum[q] += v[q];
+            if (!dz) continue;
+            if (whole) {
+                uint32_t w[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) w[q] = pack<HALF>(v[2 * q], v[2 * q + 1]);
+                store_words(dz + i * ld + j0, w);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (j0 + q * DJ < n) dz[i * ld + j0 + q * DJ] = from_f32<HALF>(v[q]);
+            }
+        }
     }
-    if (partial) partial[blockIdx.y * n + j] = sum;
+    if (!partial) return;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) sums[warp][(VEC ? lane * 8 : lane) + q * DJ] = sum[q];
+    __syncthreads();
+    const uint64_t j = blockIdx.x * (uint64_t)DZ_COLS + threadIdx.x;
+    if (j >= n) return;
+    float total = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < DZ_WARPS; ++w) total += sums[w][threadIdx.x];
+    partial[blockIdx.y * n + j] = total;
 }
 
+// db from the partial sums: a block takes 32 columns, each warp every eighth block row.
+template <bool HALF>
 __global__ void __launch_bounds__(256) db_kernel(const float* __restrict__ partial, uint64_t blocks, uint64_t n,
-                                                 int half, uint16_t* __restrict__ db, int64_t stride) {
-    const uint64_t j = blockIdx.x * 256ull + threadIdx.x;
-    if (j >= n) return;
+                                                 uint16_t* __restrict__ db, int64_t stride) {
+    __shared__ float sums[8][32];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t j = blockIdx.x * 32ull + lane;
     float sum = 0.0f;
-    for (uint64_t b = 0; b < blocks; ++b) sum += partial[b * n + j];
-    db[(int64_t)j * stride] = from_f32(sum, half);
+    if (j < n)
+        for (uint64_t b = warp; b < blocks; b += 8) sum += partial[b * n + j];
+    sums[warp][lane] = sum;
+    __syncthreads();
+    if (warp || j >= n) return;
+    float total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) total += sums[w][lane];
+    db[(int64_t)j * stride] = from_f32<HALF>(total);
 }
 
 // ---- host side -----------------------------------------------------------------------------------
@@ -466,17 +925,17 @@ static CUtensorMap operand_map(const Operand& o, int half, uint32_t box_rows) {
     return map;
 }
 
-template <int BQ, int STAGES, int CTAS>
+template <bool HALF, int BQ, int STAGES, int CTAS>
 static void launch_tile(const Operand& p, const Operand& q, const Epilogue& e, cudaStream_t st) {
     constexpr uint32_t SMEM = STAGES * (P_BYTES + BQ * BK * 2) + 256 + 1024;
-    auto* kernel = product_kernel<BQ, STAGES, CTAS>;
+    auto* kernel = product_kernel<HALF, BQ, STAGES, CTAS>;
     Product pr;
     pr.tiles_p = (uint32_t)((e.cols + BP - 1) / BP);
     pr.num_kb = (uint32_t)((p.red + BK - 1) / BK);
     pr.p_mn = p.mn;
     pr.q_mn = q.mn;
     // kind::f16: 32-bit sums, A and B of one type, their majors, N = BQ, M = 128
-    const uint32_t type = e.half ? 0u : 1u;
+    const uint32_t type = HALF ? 0u : 1u;
     pr.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)p.mn << 15) | ((uint32_t)q.mn << 16) |
                ((BQ >> 3) << 17) | ((BP >> 4) << 24);
     const uint64_t tiles = (uint64_t)pr.tiles_p * ((e.rows + BQ - 1) / BQ);
@@ -485,7 +944,7 @@ static void launch_tile(const Operand& p, const Operand& q, const Epilogue& e, c
     uint32_t split = 1;
     while (split < MAX_SPLIT && tiles * split * 2 <= 148 * CTAS && pr.num_kb / (split * 2) >= 4) split *= 2;
     if (tiles * split >= (1ull << 31)) throw Error(OZTT_EINVAL, "linear: problem too large");
-    const CUtensorMap tp = operand_map(p, e.half, BP), tq = operand_map(q, e.half, BQ);
+    const CUtensorMap tp = operand_map(p, HALF, BP), tq = operand_map(q, HALF, BQ);
     OZTT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * split), 1, 1);
@@ -502,7 +961,29 @@ static void launch_tile(const Operand& p, const Operand& q, const Epilogue& e, c
     OZTT_CUDA(cudaLaunchKernelEx(&cfg, kernel, tp, tq, pr, e, error_word()));
 }
 
+template <bool HALF, int BQ>
+static void launch_pair(const Operand& p, const Operand& q, const Epilogue& e, cudaStream_t st) {
+    constexpr uint32_t SMEM = PAIR_STAGES_BYTES + FINISHERS * PATCH_BYTES + 256 + 1024;
+    auto* kernel = pair_product_kernel<HALF, BQ>;
+    Product pr;
+    pr.tiles_p = (uint32_t)((e.cols + 2 * BP - 1) / (2 * BP));
+    pr.num_kb = (uint32_t)((p.red + BK - 1) / BK);
+    pr.p_mn = p.mn;
+    pr.q_mn = q.mn;
+    const uint32_t type = HALF ? 0u : 1u;
+    pr.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)p.mn << 15) | ((uint32_t)q.mn << 16) |
+               ((BQ >> 3) << 17) | (((2 * BP) >> 4) << 24);
+    const uint64_t tiles_q = (e.rows + BQ - 1) / BQ, tiles = pr.tiles_p * tiles_q;
+    if (tiles >= (1ull << 31)) throw Error(OZTT_EINVAL, "linear: problem too large");
+    const CUtensorMap tp = operand_map(p, HALF, BP), tq = operand_map(q, HALF, BQ / 2);
+    OZTT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+    const unsigned grid = 2u * (unsigned)std::min<uint64_t>(tiles, 74);
+    kernel<<<grid, PAIR_THREADS, SMEM, st>>>(tp, tq, pr, (uint32_t)tiles_q, e, error_word());
+    OZTT_CUDA(cudaGetLastError());
+}
+
 // out = epilogue(Q P^T): p the operand of the output's columns, q of its rows.
+template <bool HALF>
 static void product(Operand p, Operand q, Epilogue e, cudaStream_t st) {
     if (e.rows == 0 || e.cols == 0) return;
     if (e.rows >= (1ull << 31) || e.cols >= (1ull << 31) || p.red >= (1ull << 31))
@@ -518,23 +999,30 @@ static void product(Operand p, Operand q, Epilogue e, cudaStream_t st) {
         p.ks = q.ks = 1;
         p.rows = q.rows = 1;
     }
-    const auto fits = [](const View& v) { return !v.p || (v.cs == 1 && v.rs % 4 == 0 && (reinterpret_cast<uintptr_t>(v.p) & 7) == 0); };
-    e.vec = fits(e.out) && fits(e.pre) && fits(e.res);
-    if (e.rows <= 16)
-        launch_tile<16, 6, 2>(p, q, e, st);
+    const auto takes = [&](int n) {
+        const auto fits = [n](const View& v) {
+            return !v.p || (v.cs == 1 && v.rs % n == 0 && reinterpret_cast<uintptr_t>(v.p) % (2 * n) == 0);
+        };
+        return fits(e.out) && fits(e.pre) && fits(e.res);
+    };
+    e.vec = takes(8) ? 8 : takes(4) ? 4 : 1;
+    if (p.red && e.rows > 128 && ((e.rows + 255) / 256) * ((e.cols + 255) / 256) >= 37)
+        launch_pair<HALF, 256>(p, q, e, st);
+    else if (e.rows <= 16)
+        launch_tile<HALF, 16, 6, 2>(p, q, e, st);
     else if (e.rows <= 32)
-        launch_tile<32, 5, 2>(p, q, e, st);
+        launch_tile<HALF, 32, 5, 2>(p, q, e, st);
     else if (e.rows <= 64)
-        launch_tile<64, 4, 2>(p, q, e, st);
+        launch_tile<HALF, 64, 4, 2>(p, q, e, st);
     else
-        launch_tile<128, 3, 2>(p, q, e, st);
+        launch_tile<HALF, 128, 3, 2>(p, q, e, st);
 }
 
 static View view(const oztt_view& v) { return {v.data, v.row_stride, v.col_stride}; }
 
-static int half_of(int32_t format, const char* who) {
-    if (format == OZTT_FMT_BF16) return 0;
-    if (format == OZTT_FMT_FP16) return 1;
+static bool half_of(int32_t format, const char* who) {
+    if (format == OZTT_FMT_BF16) return false;
+    if (format == OZTT_FMT_FP16) return true;
     throw Error(OZTT_EINVAL, std::string(who) + ": the format must be BF16 or FP16");
 }
 static void check_act(int32_t act, const char* who) {
@@ -549,8 +1037,8 @@ static void check_view(const oztt_view& v, bool needed, const char* what) {
     if (v.row_stride < 0 || v.col_stride < 0) throw Error(OZTT_EINVAL, std::string(what) + ": strides must not be negative");
 }
 
+template <bool HALF>
 static void forward(int device, const oztt_linear& a, cudaStream_t st) {
-    const int half = half_of(a.format, "linear");
     check_act(a.activation, "linear");
     const bool some = a.m && a.n, sum = some && a.k;
     check_view(a.x, sum, "linear: x");
@@ -571,13 +1059,12 @@ static void forward(int device, const oztt_linear& a, cudaStream_t st) {
     e.bias = a.bias.data;
     e.bias_stride = a.bias.col_stride;
     e.act = a.activation;
-    e.half = half;
-    product({a.w.data, a.n, a.k, a.w.row_stride, a.w.col_stride}, {a.x.data, a.m, a.k, a.x.row_stride, a.x.col_stride},
+    product<HALF>({a.w.data, a.n, a.k, a.w.row_stride, a.w.col_stride}, {a.x.data, a.m, a.k, a.x.row_stride, a.x.col_stride},
             e, st);
 }
 
+template <bool HALF>
 static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
-    const int half = half_of(a.format, "linear_backward");
     check_act(a.activation, "linear_backward");
     const bool act = a.activation != OZTT_ACT_NONE, mn = a.m && a.n;
     check_view(a.dy, mn, "linear_backward: dy");
@@ -592,42 +1079,47 @@ static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
     View dz = view(a.dy);
     DevBuf dz_buf(st), sums(st);
     const bool products = (a.dx.data && a.m && a.k) || (a.dw.data && a.n && a.k);
+    // enough blocks to spread over the device, at least 8 rows each and at most 512
+    const uint64_t strips = (a.n + DZ_COLS - 1) / DZ_COLS;
+    const uint32_t span = (uint32_t)std::min<uint64_t>(512, round_up(std::max<uint64_t>(1, a.m * strips / (148 * 16)), 8));
+    const uint64_t blocks = (a.m + span - 1) / span;
+    if (strips >= (1ull << 31)) throw Error(OZTT_EINVAL, "linear_backward: problem too large");
+    if (a.db.data && mn) sums.alloc(blocks * a.n * 4);
     if (mn && ((act && products) || a.db.data)) {
-        const uint64_t ld = round_up(a.n, 8), blocks = (a.m + DZ_ROWS - 1) / DZ_ROWS;
-        if (blocks > 65535 * 32768ull) throw Error(OZTT_EINVAL, "linear_backward: problem too large");
+        const uint64_t ld = round_up(a.n, 8);
         const bool store = act && products;
         if (store) dz_buf.alloc(a.m * ld * 2);
-        if (a.db.data) sums.alloc(blocks * a.n * 4);
+        const auto fits = [](const View& v) { return !v.p || (v.cs == 1 && v.rs % 8 == 0 && aligned16(v.p)); };
+        const View z = act ? view(a.pre) : View{};
+        auto* kernel = fits(dz) && fits(z) ? dz_kernel<HALF, true> : dz_kernel<HALF, false>;
         for (uint64_t b0 = 0; b0 < blocks; b0 += 65535) {  // the grid's limit of block rows
-            const uint64_t nb = std::min<uint64_t>(65535, blocks - b0), i0 = b0 * DZ_ROWS;
+            const uint64_t nb = std::min<uint64_t>(65535, blocks - b0), i0 = b0 * span;
             const auto below = [&](View v) { return View{v.p ? static_cast<uint16_t*>(v.p) + (int64_t)i0 * v.rs : nullptr, v.rs, v.cs}; };
-            dz_kernel<<<dim3((unsigned)((a.n + 255) / 256), (unsigned)nb), 256, 0, st>>>(
-                below(dz), below(view(a.pre)), a.m - i0, a.n, a.activation, half,
-                store ? dz_buf.as<uint16_t>() + i0 * ld : nullptr, ld, a.db.data ? sums.as<float>() + b0 * a.n : nullptr);
+            kernel<<<dim3((unsigned)strips, (unsigned)nb), DZ_WARPS * 32, 0, st>>>(
+                below(dz), below(z), a.m - i0, a.n, span, a.activation, store ? dz_buf.as<uint16_t>() + i0 * ld : nullptr,
+                ld, a.db.data ? sums.as<float>() + b0 * a.n : nullptr);
             OZTT_CUDA(cudaGetLastError());
         }
         if (store) dz = {dz_buf.p, (int64_t)ld, 1};
     }
     if (a.db.data && a.n) {
-        const uint64_t blocks = (a.m + DZ_ROWS - 1) / DZ_ROWS;
-        db_kernel<<<(unsigned)((a.n + 255) / 256), 256, 0, st>>>(sums.as<float>(), blocks, a.n, half,
-                                                                static_cast<uint16_t*>(a.db.data), a.db.col_stride);
+        db_kernel<HALF><<<(unsigned)((a.n + 31) / 32), 256, 0, st>>>(sums.as<float>(), a.m ? blocks : 0, a.n,
+                                                                    static_cast<uint16_t*>(a.db.data), a.db.col_stride);
         OZTT_CUDA(cudaGetLastError());
     }
     Epilogue e{};
-    e.half = half;
     e.act = OZTT_ACT_NONE;
     if (a.dx.data) {  // dx[i][t] = sum_n dz[i][n] w[n][t]
         e.rows = a.m;
         e.cols = a.k;
         e.out = view(a.dx);
-        product({a.w.data, a.k, a.n, a.w.col_stride, a.w.row_stride}, {dz.p, a.m, a.n, dz.rs, dz.cs}, e, st);
+        product<HALF>({a.w.data, a.k, a.n, a.w.col_stride, a.w.row_stride}, {dz.p, a.m, a.n, dz.rs, dz.cs}, e, st);
     }
     if (a.dw.data) {  // dw[n][t] = sum_i dz[i][n] x[i][t]
         e.rows = a.n;
         e.cols = a.k;
         e.out = view(a.dw);
-        product({a.x.data, a.k, a.m, a.x.col_stride, a.x.row_stride}, {dz.p, a.n, a.m, dz.cs, dz.rs}, e, st);
+        product<HALF>({a.x.data, a.k, a.m, a.x.col_stride, a.x.row_stride}, {dz.p, a.n, a.m, dz.cs, dz.rs}, e, st);
     }
 }
 
@@ -637,7 +1129,8 @@ static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
 extern "C" int oztt_linear_forward(int device_id, const oztt_linear* args, void* stream, char* err, size_t errlen) {
     return oztt::guarded(err, errlen, [&] {
         if (!args) throw oztt::Error(OZTT_EINVAL, "linear: no arguments");
-        oztt::layer::forward(device_id, *args, reinterpret_cast<cudaStream_t>(stream));
+        const auto run = oztt::layer::half_of(args->format, "linear") ? oztt::layer::forward<true> : oztt::layer::forward<false>;
+        run(device_id, *args, reinterpret_cast<cudaStream_t>(stream));
     });
 }
 
@@ -645,6 +1138,7 @@ extern "C" int oztt_linear_backward(int device_id, const oztt_linear_grad* args,
                                     size_t errlen) {
     return oztt::guarded(err, errlen, [&] {
         if (!args) throw oztt::Error(OZTT_EINVAL, "linear_backward: no arguments");
-        oztt::layer::backward(device_id, *args, reinterpret_cast<cudaStream_t>(stream));
+        const auto run = oztt::layer::half_of(args->format, "linear_backward") ? oztt::layer::backward<true> : oztt::layer::backward<false>;
+        run(device_id, *args, reinterpret_cast<cudaStream_t>(stream));
     });
 }

@@ -101,6 +101,23 @@ def test_forward_sizes(oztt, cuda, dtype, m, n, k):
     check_forward(oztt, x, w, None, None, "none")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(1500, 2000, 64), (2048, 2304, 200), (1281, 3001, 333), (2600, 1800, 1000),
+                                   (20000, 264, 136), (300, 9000, 72)])
+def test_forward_large(oztt, cuda, dtype, m, n, k):
+    """Outputs of many tiles, whole and ragged, with every part of the epilogue."""
+    x, w, b, r = make(m, n, k, dtype, seed=m + n + k)
+    check_forward(oztt, x, w, b, r, "gelu_tanh", pre=True)
+    check_forward(oztt, x, w, b, r[:, :1].expand(m, n), "relu")
+    check_forward(oztt, x, w, None, None, "none")
+
+
+@pytest.mark.parametrize("layout", ["transposed", "padded", "odd offset"])
+def test_forward_large_layouts(oztt, cuda, layout):
+    x, w, b, r = make(1700, 2100, 264, torch.bfloat16, seed=2, layout=layout)
+    check_forward(oztt, x, w, b, r.t().contiguous().t(), "silu", pre=True)
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_forward_activations(oztt, cuda, act, dtype):
@@ -221,6 +238,15 @@ def test_backward_sizes(oztt, cuda, act, dtype, m, n, k):
     x, w, b, dy = make(m, n, k, dtype, seed=m)
     z = (2 * dy.float().roll(1, 0) * dy.float().roll(1, 1)).to(dtype)
     check_backward(oztt, dy, x, w, z if act != "none" else None, act)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(1500, 2000, 1700), (2048, 256, 2304), (1281, 3001, 1333), (5000, 520, 2600)])
+def test_backward_large(oztt, cuda, dtype, m, n, k):
+    x, w, b, dy = make(m, n, k, dtype, seed=m)
+    z = (2 * dy.float().roll(1, 0) * dy.float().roll(1, 1)).to(dtype)
+    check_backward(oztt, dy, x, w, z, "gelu_tanh")
+    check_backward(oztt, dy, x, w, None, "none")
 
 
 @pytest.mark.parametrize("layout", ["transposed", "padded", "odd offset", "every second"])
