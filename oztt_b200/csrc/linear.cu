@@ -18,6 +18,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <deque>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -56,57 +57,99 @@ struct Epilogue {
 };
 
 // ---- activations in 32 bits ----------------------------------------------------------------------
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// On pairs of values (one instruction of the packed FP32 pipe each), with the two special functions 2^x and 1/x by
+// the hardware's approximations (2^-22): a pass over dz issues 10 instructions an element so, 26 with scalar ones.
+__device__ __forceinline__ f32x2 times2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 exp2_2(f32x2 x) {
+    float a, b;
+    unpk2(x, a, b);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+    return pk2(a, b);
+}
+__device__ __forceinline__ f32x2 reciprocal2(f32x2 x) {
+    float a, b;
+    unpk2(x, a, b);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+    return pk2(a, b);
+}
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTanhScale = 0.7978845608028654f;  // sqrt(2/pi)
 constexpr float kTanhCube = 0.044715f;
+
+// 1 / (1 + 2^x): the logistic function of -x ln 2
+__device__ __forceinline__ f32x2 logistic2(f32x2 x) { return reciprocal2(add2(splat2(1.0f), exp2_2(x))); }
 
 // The normal distribution's cumulative function, and e = exp(-z^2 / 2) on the way: the rational approximation
 // 7.1.26 of Abramowitz and Stegun's Handbook of Mathematical Functions (erfc x = t (a1 + t (a2 + ...)) exp(-x^2),
 // t = 1 / (1 + p x), off by at most 1.5e-7, which the 16-bit results do not show). It has no branch and, formed
 // for the lower tail, no cancellation.
-__device__ __forceinline__ float normal_cdf(float z, float& e) {
-    const float x = fabsf(z) * 0.70710678118654752f;
-    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
-    float q = fmaf(1.061405429f, t, -1.453152027f);
-    q = fmaf(q, t, 1.421413741f);
-    q = fmaf(q, t, -0.284496736f);
-    q = fmaf(q, t, 0.254829592f);
-    e = __expf(-x * x);
-    const float tail = 0.5f * q * t * e;
-    return z < 0.0f ? tail : 1.0f - tail;
+__device__ __forceinline__ f32x2 normal_cdf2(f32x2 z, f32x2& e) {
+    const f32x2 size = z & 0x7FFFFFFF7FFFFFFFull;
+    const f32x2 t = reciprocal2(fma2(splat2(0.3275911f * 0.70710678118654752f), size, splat2(1.0f)));
+    f32x2 q = fma2(splat2(0.5f * 1.061405429f), t, splat2(0.5f * -1.453152027f));
+    q = fma2(q, t, splat2(0.5f * 1.421413741f));
+    q = fma2(q, t, splat2(0.5f * -0.284496736f));
+    q = fma2(q, t, splat2(0.5f * 0.254829592f));
+    e = exp2_2(times2(times2(z, splat2(-0.5f * kLog2e)), z));
+    float tail0, tail1, z0, z1;
+    unpk2(times2(times2(q, t), e), tail0, tail1);
+    unpk2(z, z0, z1);
+    return pk2(z0 < 0.0f ? tail0 : 1.0f - tail0, z1 < 0.0f ? tail1 : 1.0f - tail1);
 }
 
-// gelu_tanh is z (1 + tanh u) / 2 = z sigmoid(2u): no cancellation in the lower tail.
-__device__ __forceinline__ float activate(float z, int act) {
-    switch (act) {
-        case OZTT_ACT_RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
-        case OZTT_ACT_GELU: {
-            float e;
-            return z * normal_cdf(z, e);
-        }
-        case OZTT_ACT_GELU_TANH: return z * sigmoid(2.0f * kTanhScale * z * fmaf(kTanhCube * z, z, 1.0f));
-        case OZTT_ACT_SILU: return z * sigmoid(z);
-        default: return z;
+// gelu_tanh is z (1 + tanh u) / 2 = z / (1 + exp(-2u)): no cancellation in the lower tail.
+template <int ACT>
+__device__ __forceinline__ f32x2 activate2(f32x2 z) {
+    if constexpr (ACT == OZTT_ACT_RELU) {
+        float a, b;
+        unpk2(z, a, b);
+        asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(a));
+        asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(b));
+        return pk2(a, b);
+    } else if constexpr (ACT == OZTT_ACT_GELU) {
+        f32x2 e;
+        return times2(z, normal_cdf2(z, e));
+    } else if constexpr (ACT == OZTT_ACT_GELU_TANH) {
+        constexpr float c = -2.0f * kTanhScale * kLog2e;
+        return times2(z, logistic2(times2(z, fma2(splat2(c * kTanhCube), times2(z, z), splat2(c)))));
+    } else if constexpr (ACT == OZTT_ACT_SILU) {
+        return times2(z, logistic2(times2(z, splat2(-kLog2e))));
     }
+    return z;
 }
-__device__ __forceinline__ float slope(float z, int act) {
-    switch (act) {
-        case OZTT_ACT_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-        case OZTT_ACT_GELU: {
-            float e;
-            const float c = normal_cdf(z, e);
-            return fmaf(z * 0.3989422804014327f, e, c);
+// dz of a pair: dy times the activation's derivative at z.
+template <int ACT>
+__device__ __forceinline__ f32x2 through_slope2(f32x2 dy, f32x2 z) {
+    if constexpr (ACT == OZTT_ACT_RELU) {
+        float d0, d1, z0, z1;
+        unpk2(dy, d0, d1);
+        unpk2(z, z0, z1);
+        return pk2(z0 > 0.0f ? d0 : 0.0f * d0, z1 > 0.0f ? d1 : 0.0f * d1);
+    } else if constexpr (ACT == OZTT_ACT_GELU) {
+        f32x2 e;
+        const f32x2 c = normal_cdf2(z, e);
+        return times2(dy, fma2(times2(z, splat2(0.3989422804014327f)), e, c));
+    } else if constexpr (ACT == OZTT_ACT_GELU_TANH || ACT == OZTT_ACT_SILU) {
+        // z s(u) with s the logistic function: s + z u' s (1 - s) = s (1 + z u' (1 - s))
+        f32x2 s, zu;
+        if constexpr (ACT == OZTT_ACT_SILU) {
+            s = logistic2(times2(z, splat2(-kLog2e)));
+            zu = z;
+        } else {
+            constexpr float c = -2.0f * kTanhScale * kLog2e;
+            const f32x2 zz = times2(z, z);
+            s = logistic2(times2(z, fma2(splat2(c * kTanhCube), zz, splat2(c))));
+            zu = times2(z, fma2(splat2(6.0f * kTanhScale * kTanhCube), zz, splat2(2.0f * kTanhScale)));
         }
-        case OZTT_ACT_GELU_TANH: {
-            const float zz = z * z, s = sigmoid(2.0f * kTanhScale * z * fmaf(kTanhCube, zz, 1.0f));
-            return s + 2.0f * z * s * (1.0f - s) * kTanhScale * fmaf(3.0f * kTanhCube, zz, 1.0f);
-        }
-        case OZTT_ACT_SILU: {
-            const float s = sigmoid(z);
-            return s * (1.0f + z * (1.0f - s));
-        }
-        default: return 1.0f;
+        return times2(times2(dy, s), fma2(zu, sub2(splat2(1.0f), s), splat2(1.0f)));
     }
+    return dy;
 }
 
 // FP16 (HALF) or BF16 values by their bits; a pair has its first value in the low half.
@@ -119,17 +162,18 @@ __device__ __forceinline__ uint16_t from_f32(float v) {
     return HALF ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
 template <bool HALF>
-__device__ __forceinline__ void unpack(uint32_t w, float& lo, float& hi) {
+__device__ __forceinline__ f32x2 unpack(uint32_t w) {
     if (HALF) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-        lo = f.x, hi = f.y;
-    } else {
-        lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xFFFF0000u);
+        return pk2(f.x, f.y);
     }
+    return pk2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 template <bool HALF>
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+__device__ __forceinline__ uint32_t pack(f32x2 v) {
     uint32_t w;
+    float lo, hi;
+    unpk2(v, lo, hi);
     if (HALF)
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
     else
@@ -157,10 +201,31 @@ __device__ __forceinline__ void store_words(uint16_t* p, const uint32_t (&w)[4])
 
 // ---- the tile product ----------------------------------------------------------------------------
 struct Product {
-    uint32_t tiles_p, num_kb;            // tiles along the output's columns; 64-element blocks of the reduction
+    CUtensorMap p, q;
+    Epilogue e;
+    uint32_t tiles_p, tiles_q, num_kb;   // tiles along the output's columns and rows; 64-element blocks to sum
     uint32_t idesc;
     uint32_t p_mn, q_mn;                 // 1: the operand is MN-major
 };
+// One or two products of one launch (dx and dw of a backward pass): the tiles of the first, then the second's.
+template <int COUNT>
+struct Products {
+    Product of[COUNT];
+    uint32_t tiles0, tiles;              // the first's, and all
+    // the product of a tile, whose number becomes one among the product's own
+    __device__ __forceinline__ const Product& at(uint32_t& tile) const {
+        if (COUNT == 1 || tile < tiles0) return of[0];
+        tile -= tiles0;
+        return of[COUNT - 1];
+    }
+};
+
+// Lets the next kernel of the stream start while this one ends, and waits for the one before, which must be over
+// before anything in memory is read or written (both do nothing where the launch did not ask for the overlap).
+__device__ __forceinline__ void overlap_launches() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 __device__ __forceinline__ void tma_load_2d(const CUtensorMap* map, uint32_t dst, uint64_t* bar, int32_t c0,
                                             int32_t c1) {
@@ -216,28 +281,13 @@ __device__ __forceinline__ void load_operand(const CUtensorMap* map, uint32_t ds
     }
 }
 
-// The sums of N values through the activation: the choice is made once for the N.
+// 2 N sums through the activation: the choice is made once for all.
 template <int N>
-__device__ __forceinline__ void activate_all(float (&z)[N], int act) {
+__device__ __forceinline__ void activate_all(f32x2 (&z)[N], int act) {
     switch (act) {
 #define OZTT_CASE(A) \
     case A:          \
-        _Pragma("unroll") for (int q = 0; q < N; ++q) z[q] = activate(z[q], A); \
-        break;
-        OZTT_CASE(OZTT_ACT_RELU)
-        OZTT_CASE(OZTT_ACT_GELU)
-        OZTT_CASE(OZTT_ACT_GELU_TANH)
-        OZTT_CASE(OZTT_ACT_SILU)
-#undef OZTT_CASE
-        default: break;
-    }
-}
-
-__device__ __forceinline__ void slope_all(float (&z)[8], int act) {
-    switch (act) {
-#define OZTT_CASE(A) \
-    case A:          \
-        _Pragma("unroll") for (int q = 0; q < 8; ++q) z[q] = slope(z[q], A); \
+        _Pragma("unroll") for (int q = 0; q < N; ++q) z[q] = activate2<A>(z[q]); \
         break;
         OZTT_CASE(OZTT_ACT_RELU)
         OZTT_CASE(OZTT_ACT_GELU)
@@ -252,50 +302,60 @@ __device__ __forceinline__ uint16_t* element(const View& v, uint64_t i, uint64_t
     return reinterpret_cast<uint16_t*>(v.p) + (int64_t)i * v.rs + (int64_t)j * v.cs;
 }
 
-// Activation, residual and the stores of N neighbouring columns, their bias added: every one of them exists, and the
-// views take accesses of N values. out, pre (or null): where they go; r: the residual's words, if has_res.
+// Activation, residual and the stores of 2 N neighbouring columns, their bias added: every one of them exists, and the
+// views take accesses of so many values. out, pre (or null): where they go; r: the residual's words, if has_res.
 template <bool HALF, int N>
-__device__ __forceinline__ void finish_vector(uint16_t* out, uint16_t* pre, bool has_res, int act, float (&z)[N],
-                                              const uint32_t (&r)[N / 2]) {
-    uint32_t w[N / 2];
+__device__ __forceinline__ void finish_vector(uint16_t* out, uint16_t* pre, bool has_res, int act, f32x2 (&z)[N],
+                                              const uint32_t (&r)[N]) {
+    uint32_t w[N];
     if (pre) {
 #pragma unroll
-        for (int q = 0; q < N / 2; ++q) w[q] = pack<HALF>(z[2 * q], z[2 * q + 1]);
+        for (int q = 0; q < N; ++q) w[q] = pack<HALF>(z[q]);
         store_words(pre, w);
     }
     activate_all<N>(z, act);
     if (has_res) {
 #pragma unroll
-        for (int q = 0; q < N / 2; ++q) {
-            float lo, hi;
-            unpack<HALF>(r[q], lo, hi);
-            z[2 * q] += lo, z[2 * q + 1] += hi;
-        }
+        for (int q = 0; q < N; ++q) z[q] = add2(z[q], unpack<HALF>(r[q]));
     }
 #pragma unroll
-    for (int q = 0; q < N / 2; ++q) w[q] = pack<HALF>(z[2 * q], z[2 * q + 1]);
+    for (int q = 0; q < N; ++q) w[q] = pack<HALF>(z[q]);
     store_words(out, w);
 }
 // The same for any N values, (di, dj) apart, of which those inside the output are finished, by accesses of one value.
 template <bool HALF, int N>
 __device__ __forceinline__ void finish_scattered(const Epilogue& e, uint64_t i, uint64_t j, uint32_t di, uint32_t dj,
-                                                 float (&z)[N]) {
-    uint16_t r[N];
-    bool in[N];
+                                                 const float (&sums)[N]) {
+    uint16_t r[N + 1];
+    bool in[N + 1];
+    f32x2 z[(N + 1) / 2];
 #pragma unroll
     for (int q = 0; q < N; ++q) {
         in[q] = i + q * di < e.rows && j + q * dj < e.cols;
         r[q] = e.res.p && in[q] ? *element(e.res, i + q * di, j + q * dj) : 0;
     }
-    if (e.pre.p) {
+    in[N] = false;
 #pragma unroll
-        for (int q = 0; q < N; ++q)
-            if (in[q]) *element(e.pre, i + q * di, j + q * dj) = from_f32<HALF>(z[q]);
+    for (int q = 0; q < (N + 1) / 2; ++q) z[q] = pk2(sums[2 * q], 2 * q + 1 < N ? sums[2 * q + 1 < N ? 2 * q + 1 : 0] : 0.0f);
+    const auto store = [&](const View& v) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            const uint32_t w = pack<HALF>(z[q / 2]);
+            if (in[q]) *element(v, i + q * di, j + q * dj) = (uint16_t)(w >> (16 * (q & 1)));
+        }
+    };
+    if (e.pre.p) store(e.pre);
+    activate_all(z, e.act);
+    if (e.res.p) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            float lo, hi;
+            unpk2(z[q / 2], lo, hi);
+            const float y = ((q & 1) ? hi : lo) + to_f32<HALF>(r[q]);
+            z[q / 2] = (q & 1) ? pk2(lo, y) : pk2(y, hi);
+        }
     }
-    activate_all<N>(z, e.act);
-#pragma unroll
-    for (int q = 0; q < N; ++q)
-        if (in[q]) *element(e.out, i + q * di, j + q * dj) = from_f32<HALF>(e.res.p ? z[q] + to_f32<HALF>(r[q]) : z[q]);
+    store(e.out);
 }
 template <bool HALF>
 __device__ __forceinline__ float bias_at(const Epilogue& e, uint64_t j) {
@@ -306,10 +366,9 @@ __device__ __forceinline__ float bias_at(const Epilogue& e, uint64_t j) {
 // sums its stretch of it in tensor memory and lays the 32-bit sums down in its own shared memory (where the
 // operand stages were), then each finishes its share of the rows, adding the stretches in the cluster's order
 // through distributed shared memory, so the result does not depend on timing.
-template <bool HALF, int BQ, int STAGES, int CTAS>
+template <bool HALF, int COUNT, int BQ, int STAGES, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS)
-    product_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ, const Product pr,
-                   const Epilogue e, int* err) {
+    product_kernel(const __grid_constant__ Products<COUNT> ps, int* err) {
     constexpr uint32_t Q_BYTES = BQ * BK * 2;
     constexpr uint32_t STAGE_BYTES = P_BYTES + Q_BYTES;
     constexpr uint32_t TMEM_COLS = BQ < 32 ? 32 : BQ;
@@ -326,8 +385,11 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     uint32_t split;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(split));
     const uint32_t rank = cluster_rank();
-    const uint32_t tile = blockIdx.x / split;
+    uint32_t tile = blockIdx.x / split;
+    const Product& pr = ps.at(tile);
+    const Epilogue& e = pr.e;
     const uint32_t tp = tile % pr.tiles_p, tq = tile / pr.tiles_p;
+    const uint32_t p_mn = pr.p_mn, q_mn = pr.q_mn;
     const uint32_t kb0 = (uint32_t)((uint64_t)pr.num_kb * rank / split);
     const uint32_t kb1 = (uint32_t)((uint64_t)pr.num_kb * (rank + 1) / split);
 
@@ -351,6 +413,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    overlap_launches();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -363,8 +426,8 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                 }
                 mbar_expect_tx(full_bar + stage, STAGE_BYTES);
                 const uint32_t sp = smem_u32(smem + stage * STAGE_BYTES);
-                load_operand(&tmP, sp, full_bar + stage, (int32_t)(tp * BP), (int32_t)(kb * BK), BP, pr.p_mn);
-                load_operand(&tmQ, sp + P_BYTES, full_bar + stage, (int32_t)(tq * BQ), (int32_t)(kb * BK), BQ, pr.q_mn);
+                load_operand(&pr.p, sp, full_bar + stage, (int32_t)(tp * BP), (int32_t)(kb * BK), BP, p_mn);
+                load_operand(&pr.q, sp + P_BYTES, full_bar + stage, (int32_t)(tq * BQ), (int32_t)(kb * BK), BQ, q_mn);
                 filled |= 1u << stage;
                 last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
                 if (++stage == STAGES) {
@@ -379,15 +442,15 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     } else if (warp == 1) {
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
-            const uint32_t step_p = pr.p_mn ? UK * 128u : UK * 2u, step_q = pr.q_mn ? UK * 128u : UK * 2u;
+            const uint32_t step_p = p_mn ? UK * 128u : UK * 2u, step_q = q_mn ? UK * 128u : UK * 2u, idesc = pr.idesc;
             for (uint32_t kb = kb0; kb < kb1; ++kb) {
                 if (!mbar_wait(full_bar + stage, phase, abort_flag, err, ERR_WAIT_MMA_FULL)) break;
                 tc_fence_after();
                 const uint32_t sp = smem_u32(smem + stage * STAGE_BYTES), sq = sp + P_BYTES;
 #pragma unroll
                 for (uint32_t k = 0; k < BK / UK; ++k)
-                    umma_16(tmem_base, operand_desc(sp + k * step_p, pr.p_mn), operand_desc(sq + k * step_q, pr.q_mn),
-                            pr.idesc, kb != kb0 || k != 0);
+                    umma_16(tmem_base, operand_desc(sp + k * step_p, p_mn), operand_desc(sq + k * step_q, q_mn), idesc,
+                            kb != kb0 || k != 0);
                 umma_commit(empty_bar + stage);
                 if (++stage == STAGES) {
                     stage = 0;
@@ -448,9 +511,9 @@ __global__ void __launch_bounds__(THREADS, CTAS)
                 const float4 v = ld_cluster_f4(map_to(row + lane * 16, c));
                 acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
             }
-            z[0] += acc.x, z[1] += acc.y, z[2] += acc.z, z[3] += acc.w;
-            finish_vector<HALF, 4>(element(e.out, i, col[0]), e.pre.p ? element(e.pre, i, col[0]) : nullptr, e.res.p, e.act,
-                                   z, res);
+            f32x2 sum[2] = {pk2(z[0] + acc.x, z[1] + acc.y), pk2(z[2] + acc.z, z[3] + acc.w)};
+            finish_vector<HALF, 2>(element(e.out, i, col[0]), e.pre.p ? element(e.pre, i, col[0]) : nullptr, e.res.p, e.act,
+                                   sum, res);
         } else {
             float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             for (uint32_t c = 0; c < split; ++c) {
@@ -515,18 +578,21 @@ __device__ __forceinline__ void umma_16_pair(uint32_t d_tmem, uint64_t adesc, ui
         : "memory");
 }
 
-// Tile number -> tile column tp, tile row tq: groups of GROUP_Q tile rows, each walked column by column.
-__device__ __forceinline__ void tile_at(uint32_t tile, uint32_t tiles_p, uint32_t tiles_q, uint32_t& tp, uint32_t& tq) {
-    const uint32_t span = GROUP_Q * tiles_p, g = tile / span, first = g * GROUP_Q;
-    const uint32_t size = min(tiles_q - first, GROUP_Q), r = tile - g * span;
+// Tile number -> its product, tile column tp and tile row tq: groups of GROUP_Q tile rows, each walked column by
+// column.
+template <int COUNT>
+__device__ __forceinline__ const Product& tile_at(const Products<COUNT>& ps, uint32_t tile, uint32_t& tp, uint32_t& tq) {
+    const Product& pr = ps.at(tile);
+    const uint32_t span = GROUP_Q * pr.tiles_p, g = tile / span, first = g * GROUP_Q;
+    const uint32_t size = min(pr.tiles_q - first, GROUP_Q), r = tile - g * span;
     tq = first + r % size;
     tp = r / size;
+    return pr;
 }
 
-template <bool HALF, int BQ>
+template <bool HALF, int COUNT, int BQ>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
-    pair_product_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
-                        const Product pr, const uint32_t tiles_q, const Epilogue e, int* err) {
+    pair_product_kernel(const __grid_constant__ Products<COUNT> ps, int* err) {
     constexpr uint32_t HALF_Q = BQ / 2;
     constexpr uint32_t STAGE_BYTES = P_BYTES + HALF_Q * BK * 2;
     constexpr uint32_t STAGES = PAIR_STAGES_BYTES / STAGE_BYTES;
@@ -545,7 +611,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const uint32_t first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
-    const uint32_t num_tiles = pr.tiles_p * tiles_q;
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < STAGES; ++s) {
@@ -572,15 +637,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     cluster_sync();  // the peer's barriers are initialised before anything is signalled across the pair
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    overlap_launches();
 
     if (warp == 0) {
         if (lane == 0) {
             uint32_t stage = 0, phase = 0, filled = 0, last_phase = 0;
             bool ok = true, issued = false;
-            for (uint32_t tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
+            for (uint32_t tile = first_tile; ok && tile < ps.tiles; tile += tile_step) {
                 uint32_t tp, tq;
-                tile_at(tile, pr.tiles_p, tiles_q, tp, tq);
-                for (uint32_t kb = 0; kb < pr.num_kb; ++kb) {
+                const Product& pr = tile_at(ps, tile, tp, tq);
+                const uint32_t num_kb = pr.num_kb, p_mn = pr.p_mn, q_mn = pr.q_mn;
+                const CUtensorMap *map_p = &pr.p, *map_q = &pr.q;
+                for (uint32_t kb = 0; kb < num_kb; ++kb) {
                     if (!mbar_wait(empty_bar + stage, phase ^ 1u, abort_flag, err, ERR_WAIT_PRODUCER)) {
                         ok = false;
                         break;
@@ -588,10 +656,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     if (rank == 0) mbar_expect_tx(full_bar + stage, 2 * STAGE_BYTES);
                     const uint32_t full_leader = map_to(smem_u32(full_bar + stage), 0);
                     const uint32_t sp = smem_u32(smem + stage * STAGE_BYTES);
-                    load_operand_pair(&tmP, sp, full_leader, (int32_t)(tp * 2 * BP + rank * BP), (int32_t)(kb * BK), BP,
-                                      pr.p_mn);
-                    load_operand_pair(&tmQ, sp + P_BYTES, full_leader, (int32_t)(tq * BQ + rank * HALF_Q),
-                                      (int32_t)(kb * BK), HALF_Q, pr.q_mn);
+                    load_operand_pair(map_p, sp, full_leader, (int32_t)(tp * 2 * BP + rank * BP), (int32_t)(kb * BK), BP,
+                                      p_mn);
+                    load_operand_pair(map_q, sp + P_BYTES, full_leader, (int32_t)(tq * BQ + rank * HALF_Q),
+                                      (int32_t)(kb * BK), HALF_Q, q_mn);
                     issued = true;
                     filled |= 1u << stage;
                     last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
@@ -615,13 +683,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
-            const uint32_t step_p = pr.p_mn ? UK * 128u : UK * 2u, step_q = pr.q_mn ? UK * 128u : UK * 2u;
             bool ok = true;
-            for (uint32_t tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
+            for (uint32_t tile = first_tile; ok && tile < ps.tiles; tile += tile_step) {
+                uint32_t own = tile;
+                const Product& pr = ps.at(own);
+                const uint32_t num_kb = pr.num_kb, p_mn = pr.p_mn, q_mn = pr.q_mn, idesc = pr.idesc;
+                const uint32_t step_p = p_mn ? UK * 128u : UK * 2u, step_q = q_mn ? UK * 128u : UK * 2u;
                 if (!mbar_wait(tempty_bar + acc, acc_phase ^ 1u, abort_flag, err, ERR_WAIT_MMA_EMPTY)) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * BQ;
-                for (uint32_t kb = 0; kb < pr.num_kb; ++kb) {
+                for (uint32_t kb = 0; kb < num_kb; ++kb) {
                     if (!mbar_wait(full_bar + stage, phase, abort_flag, err, ERR_WAIT_MMA_FULL)) {
                         ok = false;
                         break;
@@ -630,8 +701,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     const uint32_t sp = smem_u32(smem + stage * STAGE_BYTES), sq = sp + P_BYTES;
 #pragma unroll
                     for (uint32_t k = 0; k < BK / UK; ++k)
-                        umma_16_pair(d_tmem, operand_desc(sp + k * step_p, pr.p_mn),
-                                     operand_desc(sq + k * step_q, pr.q_mn), pr.idesc, (kb | k) != 0u);
+                        umma_16_pair(d_tmem, operand_desc(sp + k * step_p, p_mn),
+                                     operand_desc(sq + k * step_q, q_mn), idesc, (kb | k) != 0u);
                     const uint32_t eb = smem_u32(empty_bar + stage);
                     umma_commit_pair(eb);
                     umma_commit_pair(map_to(eb, 1));
@@ -658,18 +729,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         float* patch = patches + (warp - 2) * (PATCH_BYTES / 4);
         const uint32_t prow = lane >> 2, pcol = (lane & 3u) * 8u;
         uint32_t acc = 0, acc_phase = 0;
-        for (uint32_t tile = first_tile; tile < num_tiles; tile += tile_step) {
+        for (uint32_t tile = first_tile; tile < ps.tiles; tile += tile_step) {
             uint32_t tp, tq;
-            tile_at(tile, pr.tiles_p, tiles_q, tp, tq);
+            const Product& pr = tile_at(ps, tile, tp, tq);
+            const Epilogue& e = pr.e;
             const uint64_t j0 = (uint64_t)tp * 2 * BP + rank * BP + quarter * 32u;
             const uint64_t i0 = (uint64_t)tq * BQ + c0;
             const bool vec = e.vec >= 8 && j0 + 32 <= e.cols;
-            float bias[8];
+            f32x2 bias[4];
+            float lane_bias = 0.0f;
             if (vec) {
 #pragma unroll
-                for (int q = 0; q < 8; ++q) bias[q] = bias_at<HALF>(e, j0 + pcol + q);
+                for (int q = 0; q < 4; ++q)
+                    bias[q] = pk2(bias_at<HALF>(e, j0 + pcol + 2 * q), bias_at<HALF>(e, j0 + pcol + 2 * q + 1));
             } else {
-                bias[0] = bias_at<HALF>(e, j0 + lane);
+                lane_bias = bias_at<HALF>(e, j0 + lane);
             }
             const uint32_t rows = j0 < e.cols && i0 < e.rows ? (uint32_t)min((uint64_t)ROWS, e.rows - i0) : 0;
             // this lane's place in the first patch; the next is 8 rows further
@@ -693,11 +767,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 #pragma unroll
                     for (int q = 0; q < 8; ++q) patch[q * PATCH_LD + lane] = __uint_as_float(v[q]);
                     __syncwarp();
-                    const float4* p = reinterpret_cast<const float4*>(patch + prow * PATCH_LD + pcol);
-                    const float4 x = p[0], y = p[1];
-                    float z[8] = {x.x + bias[0], x.y + bias[1], x.z + bias[2], x.w + bias[3],
-                                  y.x + bias[4], y.y + bias[5], y.z + bias[6], y.w + bias[7]};
-                    if (mine) finish_vector<HALF, 8>(out, has_pre ? pre : nullptr, has_res, e.act, z, r);
+                    const ulonglong2* p = reinterpret_cast<const ulonglong2*>(patch + prow * PATCH_LD + pcol);
+                    const ulonglong2 x = p[0], y = p[1];
+                    f32x2 z[4] = {add2(x.x, bias[0]), add2(x.y, bias[1]), add2(y.x, bias[2]), add2(y.y, bias[3])};
+                    if (mine) finish_vector<HALF, 4>(out, has_pre ? pre : nullptr, has_res, e.act, z, r);
                     out += PATCH_ROWS * e.out.rs;
                     pre += PATCH_ROWS * e.pre.rs;
                     res += PATCH_ROWS * e.res.rs;
@@ -709,7 +782,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     tmem_ld8(tbase + c, v);
                     float z[8];
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) z[q] = __uint_as_float(v[q]) + bias[0];
+                    for (int q = 0; q < 8; ++q) z[q] = __uint_as_float(v[q]) + lane_bias;
                     finish_scattered<HALF, 8>(e, i0 + c, j0 + lane, 1, 0, z);
                 }
             }
@@ -731,6 +804,93 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     }
 }
 
+// ---- few rows ------------------------------------------------------------------------------------
+// The product for up to 4 output rows (single tokens), on the 32-bit pipe: bound by the bytes of P, of which each
+// is read once, and by the time to the first of them, so nothing is set up: a warp streams 4 rows of P (VEC: 16
+// bytes a lane) along their reduction index and multiplies them by the rows of Q, which the first-level cache
+// keeps. With few rows of P the warps of a block share their reduction and join through shared memory, in order.
+constexpr int FEW_COLS = 4;  // output columns (rows of P) of a warp
+template <bool HALF, int M, bool VEC>
+__global__ void __launch_bounds__(256)
+    few_rows_kernel(const uint16_t* __restrict__ p, int64_t ldp, const uint16_t* __restrict__ q, int64_t ldq,
+                    const uint32_t red, const __grid_constant__ Epilogue e) {
+    __shared__ float sums[8][FEW_COLS * M];
+    constexpr uint32_t STEP = VEC ? 256 : 32;  // reduction elements of a warp's access
+    constexpr int AHEAD = VEC ? 2 : M > 2 ? 4 : 8;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const uint64_t j0 = blockIdx.x * (uint64_t)FEW_COLS;
+    overlap_launches();
+    const uint16_t* row[FEW_COLS];  // columns past the last one read it again
+#pragma unroll
+    for (int c = 0; c < FEW_COLS; ++c) row[c] = p + (int64_t)min(j0 + c, e.cols - 1) * ldp;
+    f32x2 acc[M][FEW_COLS] = {};  // two sums, of every other element (access)
+    for (uint32_t t0 = warp * STEP; t0 < red; t0 += warps * STEP * AHEAD) {
+        if constexpr (VEC) {
+            uint32_t w[AHEAD][FEW_COLS][4], x[AHEAD][M][4];
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const uint32_t t = t0 + a * warps * STEP + lane * 8;
+#pragma unroll
+                for (int c = 0; c < FEW_COLS; ++c) {
+                    w[a][c][0] = w[a][c][1] = w[a][c][2] = w[a][c][3] = 0;
+                    if (t < red) load_words(row[c] + t, w[a][c]);  // red is a multiple of 8
+                }
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    x[a][m][0] = x[a][m][1] = x[a][m][2] = x[a][m][3] = 0;
+                    if (t < red) load_words(q + m * ldq + t, x[a][m]);
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a)
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+#pragma unroll
+                    for (int c = 0; c < FEW_COLS; ++c) {
+                        const f32x2 v = unpack<HALF>(w[a][c][h]);
+#pragma unroll
+                        for (int m = 0; m < M; ++m) acc[m][c] = fma2(v, unpack<HALF>(x[a][m][h]), acc[m][c]);
+                    }
+        } else {
+            uint16_t w[AHEAD][FEW_COLS], x[AHEAD][M];
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const uint32_t t = t0 + a * warps * STEP + lane;
+#pragma unroll
+                for (int c = 0; c < FEW_COLS; ++c) w[a][c] = t < red ? row[c][t] : 0;
+#pragma unroll
+                for (int m = 0; m < M; ++m) x[a][m] = t < red ? q[m * ldq + t] : 0;
+            }
+#pragma unroll
+            for (int a = 0; a < AHEAD; a += 2)
+#pragma unroll
+                for (int c = 0; c < FEW_COLS; ++c)
+#pragma unroll
+                    for (int m = 0; m < M; ++m)
+                        acc[m][c] = fma2(pk2(to_f32<HALF>(w[a][c]), to_f32<HALF>(w[a + 1][c])),
+                                         pk2(to_f32<HALF>(x[a][m]), to_f32<HALF>(x[a + 1][m])), acc[m][c]);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int c = 0; c < FEW_COLS; ++c) {
+            float even, odd;
+            unpk2(acc[m][c], even, odd);
+            even += odd;
+#pragma unroll
+            for (int d = 16; d; d >>= 1) even += __shfl_xor_sync(0xFFFFFFFFu, even, d);
+            if (lane == 0) sums[warp][m * FEW_COLS + c] = even;
+        }
+    __syncthreads();
+    if (threadIdx.x < FEW_COLS * M) {
+        const uint64_t i = threadIdx.x / FEW_COLS, j = j0 + threadIdx.x % FEW_COLS;
+        float z[1] = {bias_at<HALF>(e, j)};
+        for (uint32_t w = 0; w < warps; ++w) z[0] += sums[w][threadIdx.x];
+        finish_scattered<HALF, 1>(e, i, j, 0, 0, z);
+    }
+}
+
 // ---- passes over memory --------------------------------------------------------------------------
 
 // dst[o][i] = src[o * so + i * si], rows ld apart (ld a multiple of 8, zero beyond `inner`): operands whose base
@@ -739,6 +899,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint16_t* __restrict__ 
                                                    uint64_t outer, uint64_t inner, uint16_t* __restrict__ dst,
                                                    uint64_t ld) {
     const uint64_t per_row = ld / 8, count = outer * per_row;
+    overlap_launches();
     for (uint64_t t = blockIdx.x * (uint64_t)blockDim.x + threadIdx.x; t < count; t += (uint64_t)gridDim.x * blockDim.x) {
         const uint64_t o = t / per_row, i = (t - o * per_row) * 8;
         uint32_t w[4];
@@ -753,95 +914,117 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint16_t* __restrict__ 
     }
 }
 
-// dz = dy * act'(z) into dz (rows ld apart; may be null), and the sums of its columns over this block's rows in
-// 32 bits into partial[block row][n] (may be null), always in the same order. A block takes 256 columns by `span`
-// rows, a warp one row at a time, four rows' loads in flight. VEC: a lane takes 8 neighbouring columns by 16-byte
-// accesses, else 8 columns 32 apart.
-constexpr uint32_t DZ_COLS = 256, DZ_WARPS = 8, DZ_AHEAD = 4;
-template <bool HALF, bool VEC>
-__global__ void __launch_bounds__(DZ_WARPS * 32)
-    dz_kernel(View dy, View z, uint64_t m, uint64_t n, uint32_t span, int act, uint16_t* __restrict__ dz, uint64_t ld,
-              float* __restrict__ partial) {
-    __shared__ float sums[DZ_WARPS][DZ_COLS];
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint64_t j0 = blockIdx.x * (uint64_t)DZ_COLS + (VEC ? lane * 8 : lane);
-    const uint64_t i0 = blockIdx.y * (uint64_t)span, i1 = min(i0 + span, m);
-    const bool whole = VEC && j0 + 8 <= n;
-    constexpr uint32_t DJ = VEC ? 1 : 32;
-    float sum[8] = {};
-    for (uint64_t base = i0 + warp; base < i1; base += DZ_WARPS * DZ_AHEAD) {
-        uint32_t g[DZ_AHEAD][4], s[DZ_AHEAD][4];
+// dz = dy * act'(z) into dz (rows ld apart; may be null), and the sums of its columns in 32 bits. A block takes 64
+// columns (a lane 8 neighbouring ones by 16-byte accesses with VEC, else 8 that are 8 apart) by `span` rows, 32 at
+// a time and twice as many in flight; the blocks of a cluster lie below one another and join their sums, always
+// in the same order, through distributed shared memory: into db where one cluster covers all rows, else into
+// partial[cluster][n] for db_kernel. (db and partial may be null.)
+constexpr uint32_t DZ_COLS = 64, DZ_ROWS = 32, DZ_AHEAD = 2, DZ_CLUSTER = 8;
+template <bool HALF, bool VEC, int ACT>
+__global__ void __launch_bounds__(256, 3)
+    dz_kernel(View dy, View z, uint64_t m, uint64_t n, uint64_t span, uint16_t* __restrict__ dz, uint64_t ld,
+              float* __restrict__ partial, uint16_t* __restrict__ db, int64_t db_stride) {
+    __shared__ float sums[DZ_ROWS][DZ_COLS];
+    __shared__ float block_sums[DZ_COLS];
+    const uint32_t r = threadIdx.x >> 3, l = threadIdx.x & 7;
+    const uint32_t l0 = VEC ? l * 8 : l;
+    constexpr uint32_t DJ = VEC ? 1 : 8;
+    const uint64_t j0 = blockIdx.x * (uint64_t)DZ_COLS + l0;
+    const uint64_t i0 = min(blockIdx.y * span, m) + r, i1 = min((blockIdx.y + 1) * span, m);
+    // the columns that exist: with VEC (n a multiple of 8) all or none
+    const uint32_t cols = j0 >= n ? 0 : VEC ? 8 : (uint32_t)min((n - j0 + 7) / 8, (uint64_t)8);
+    overlap_launches();
+    f32x2 sum[4] = {};
+    if (cols && i0 < i1) {
+        const uint16_t *py = element(dy, i0, j0), *pz = element(z, i0, j0);
+        uint16_t* pd = dz + i0 * ld + j0;
+        const int64_t step_y = DZ_ROWS * dy.rs, step_z = DZ_ROWS * z.rs, step_d = DZ_ROWS * (int64_t)ld;
+        uint32_t left = (uint32_t)((i1 - i0 + DZ_ROWS - 1) / DZ_ROWS);  // of this thread's rows
+        while (left) {
+            uint32_t g[DZ_AHEAD][4], s[DZ_AHEAD][4];
 #pragma unroll
-        for (uint32_t a = 0; a < DZ_AHEAD; ++a) {
-            const uint64_t i = base + a * DZ_WARPS;
+            for (uint32_t a = 0; a < DZ_AHEAD; ++a) {
+                if (a >= left) break;
+                if constexpr (VEC) {
+                    load_words(py + a * step_y, g[a]);
+                    if (ACT != OZTT_ACT_NONE) load_words(pz + a * step_z, s[a]);
+                } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) g[a][q] = s[a][q] = 0;
-            if (i >= i1) continue;
-            if (whole) {
-                load_words(element(dy, i, j0), g[a]);
-                if (act != OZTT_ACT_NONE) load_words(element(z, i, j0), s[a]);
-            } else {
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const uint64_t j = j0 + q * DJ;
-                    if (j >= n) continue;
-                    g[a][q >> 1] |= (uint32_t)*element(dy, i, j) << (16 * (q & 1));
-                    if (act != OZTT_ACT_NONE) s[a][q >> 1] |= (uint32_t)*element(z, i, j) << (16 * (q & 1));
+                    for (uint32_t q = 0; q < 4; ++q) {
+                        const auto pair = [&](const uint16_t* p, int64_t cs) {
+                            return (2 * q < cols ? (uint32_t)p[(int64_t)(2 * q * DJ) * cs] : 0u) |
+                                   (2 * q + 1 < cols ? (uint32_t)p[(int64_t)((2 * q + 1) * DJ) * cs] << 16 : 0u);
+                        };
+                        g[a][q] = pair(py + a * step_y, dy.cs);
+                        if (ACT != OZTT_ACT_NONE) s[a][q] = pair(pz + a * step_z, z.cs);
+                    }
                 }
             }
-        }
 #pragma unroll
-        for (uint32_t a = 0; a < DZ_AHEAD; ++a) {
-            const uint64_t i = base + a * DZ_WARPS;
-            if (i >= i1) continue;
-            float v[8];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) unpack<HALF>(g[a][q], v[2 * q], v[2 * q + 1]);
-            if (act != OZTT_ACT_NONE) {
-                float t[8];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) unpack<HALF>(s[a][q], t[2 * q], t[2 * q + 1]);
-                slope_all(t, act);
-#pragma unroll
-                for (int q = 0; q < 8; ++q) v[q] *= t[q];
-            }
-#pragma unroll
-            for (int q = 0; q < 8; ++q) sum[q] += v[q];
-            if (!dz) continue;
-            if (whole) {
+            for (uint32_t a = 0; a < DZ_AHEAD; ++a) {
+                if (a >= left) break;
                 uint32_t w[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) w[q] = pack<HALF>(v[2 * q], v[2 * q + 1]);
-                store_words(dz + i * ld + j0, w);
-            } else {
+                for (int q = 0; q < 4; ++q) {
+                    f32x2 v = unpack<HALF>(g[a][q]);
+                    if (ACT != OZTT_ACT_NONE) v = through_slope2<ACT>(v, unpack<HALF>(s[a][q]));
+                    sum[q] = add2(sum[q], v);
+                    w[q] = pack<HALF>(v);
+                }
+                if (!dz) continue;
+                if constexpr (VEC) {
+                    store_words(pd + a * step_d, w);
+                } else {
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (j0 + q * DJ < n) dz[i * ld + j0 + q * DJ] = from_f32<HALF>(v[q]);
+                    for (uint32_t q = 0; q < 8; ++q)
+                        if (q < cols) pd[a * step_d + q * DJ] = (uint16_t)(w[q >> 1] >> (16 * (q & 1)));
+                }
             }
+            py += DZ_AHEAD * step_y;
+            pz += DZ_AHEAD * step_z;
+            pd += DZ_AHEAD * step_d;
+            left -= min(left, DZ_AHEAD);
         }
     }
-    if (!partial) return;
+    if (!partial && !db) return;  // the same for every block
 #pragma unroll
-    for (int q = 0; q < 8; ++q) sums[warp][(VEC ? lane * 8 : lane) + q * DJ] = sum[q];
+    for (int q = 0; q < 4; ++q) unpk2(sum[q], sums[r][l0 + 2 * q * DJ], sums[r][l0 + (2 * q + 1) * DJ]);
     __syncthreads();
-    const uint64_t j = blockIdx.x * (uint64_t)DZ_COLS + threadIdx.x;
-    if (j >= n) return;
-    float total = 0.0f;
-#pragma unroll
-    for (uint32_t w = 0; w < DZ_WARPS; ++w) total += sums[w][threadIdx.x];
-    partial[blockIdx.y * n + j] = total;
+    if (threadIdx.x < DZ_COLS) {
+        float total = 0.0f;
+#pragma unroll 8
+        for (uint32_t w = 0; w < DZ_ROWS; ++w) total += sums[w][threadIdx.x];
+        block_sums[threadIdx.x] = total;
+    }
+    __syncthreads();
+    cluster_sync();
+    if (cluster_rank() == 0 && threadIdx.x < DZ_COLS) {
+        uint32_t blocks;
+        asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
+        const uint64_t j = blockIdx.x * (uint64_t)DZ_COLS + threadIdx.x;
+        float total = 0.0f;
+        for (uint32_t c = 0; c < blocks; ++c) total += ld_cluster_f1(map_to(smem_u32(block_sums + threadIdx.x), c));
+        if (j < n) {
+            if (db)
+                db[(int64_t)j * db_stride] = from_f32<HALF>(total);
+            else
+                partial[blockIdx.y / blocks * n + j] = total;
+        }
+    }
+    cluster_sync();  // no block leaves while its sums may be read
 }
 
-// db from the partial sums: a block takes 32 columns, each warp every eighth block row.
+// db from the clusters' sums: a block takes 32 columns, each warp every eighth cluster.
 template <bool HALF>
-__global__ void __launch_bounds__(256) db_kernel(const float* __restrict__ partial, uint64_t blocks, uint64_t n,
+__global__ void __launch_bounds__(256) db_kernel(const float* __restrict__ partial, uint64_t clusters, uint64_t n,
                                                  uint16_t* __restrict__ db, int64_t stride) {
     __shared__ float sums[8][32];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint64_t j = blockIdx.x * 32ull + lane;
+    overlap_launches();
     float sum = 0.0f;
     if (j < n)
-        for (uint64_t b = warp; b < blocks; b += 8) sum += partial[b * n + j];
+        for (uint64_t b = warp; b < clusters; b += 8) sum += partial[b * n + j];
     sums[warp][lane] = sum;
     __syncthreads();
     if (warp || j >= n) return;
@@ -886,6 +1069,36 @@ struct Operand {
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// Launches a kernel so that it may start while the kernel before it on the stream ends (overlap_launches), its
+// blocks in clusters of `cluster` (as the kernel says where that is {0}).
+template <class... Params, class... Args>
+static void launch(void (*kernel)(Params...), dim3 grid, uint32_t threads, uint32_t smem, dim3 cluster,
+                   cudaStream_t st, Args&&... args) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster.x;
+    attr[1].val.clusterDim.y = cluster.y;
+    attr[1].val.clusterDim.z = cluster.z;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster.x ? 2 : 1;
+    OZTT_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+}
+template <class Kernel>
+static void allow_smem(Kernel* kernel, uint32_t bytes, std::atomic<uint64_t>& allowed) {
+    int device = 0;
+    OZTT_CUDA(cudaGetDevice(&device));
+    if (device < 64 && (allowed.load() >> device & 1)) return;
+    OZTT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (device < 64) allowed.fetch_or(1ull << device);
+}
+
 // The operand as the tensor copies can read it: as it lies (K-major, or MN-major where allowed), or packed.
 static void settle(Operand& o, bool allow_mn, DevBuf& buf, cudaStream_t st) {
     if (o.red == 1) o.ks = 1;  // a stride that no element uses
@@ -902,9 +1115,8 @@ static void settle(Operand& o, bool allow_mn, DevBuf& buf, cudaStream_t st) {
     const uint64_t outer = mn ? o.red : o.rows, inner = mn ? o.rows : o.red, ld = round_up(inner, 8);
     buf.alloc(outer * ld * 2);
     const unsigned grid = (unsigned)std::min<uint64_t>((outer * (ld / 8) + 255) / 256, 148 * 16);
-    pack_kernel<<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(o.p), mn ? o.ks : o.rs, mn ? o.rs : o.ks, outer,
-                                      inner, buf.as<uint16_t>(), ld);
-    OZTT_CUDA(cudaGetLastError());
+    launch(pack_kernel, dim3(grid), 256, 0, dim3(0), st, static_cast<const uint16_t*>(o.p), mn ? o.ks : o.rs,
+           mn ? o.rs : o.ks, outer, inner, buf.as<uint16_t>(), ld);
     o.p = buf.p;
     o.mn = mn;
     (mn ? o.ks : o.rs) = (int64_t)ld;
@@ -925,97 +1137,154 @@ static CUtensorMap operand_map(const Operand& o, int half, uint32_t box_rows) {
     return map;
 }
 
-template <bool HALF, int BQ, int STAGES, int CTAS>
-static void launch_tile(const Operand& p, const Operand& q, const Epilogue& e, cudaStream_t st) {
-    constexpr uint32_t SMEM = STAGES * (P_BYTES + BQ * BK * 2) + 256 + 1024;
-    auto* kernel = product_kernel<HALF, BQ, STAGES, CTAS>;
+// A product to be done: operands as the tensor copies read them, and its epilogue.
+struct Task {
+    Operand p, q;
+    Epilogue e;
+};
+
+template <bool HALF>
+static Product describe(const Task& t, uint32_t tile_p, uint32_t tile_q, uint32_t box_q) {
     Product pr;
-    pr.tiles_p = (uint32_t)((e.cols + BP - 1) / BP);
-    pr.num_kb = (uint32_t)((p.red + BK - 1) / BK);
-    pr.p_mn = p.mn;
-    pr.q_mn = q.mn;
-    // kind::f16: 32-bit sums, A and B of one type, their majors, N = BQ, M = 128
+    pr.p = operand_map(t.p, HALF, BP);
+    pr.q = operand_map(t.q, HALF, box_q);
+    pr.e = t.e;
+    pr.tiles_p = (uint32_t)((t.e.cols + tile_p - 1) / tile_p);
+    pr.tiles_q = (uint32_t)((t.e.rows + tile_q - 1) / tile_q);
+    pr.num_kb = (uint32_t)((t.p.red + BK - 1) / BK);
+    pr.p_mn = t.p.mn;
+    pr.q_mn = t.q.mn;
+    // kind::f16: 32-bit sums, A and B of one type, their majors, N = tile_q, M = tile_p
     const uint32_t type = HALF ? 0u : 1u;
-    pr.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)p.mn << 15) | ((uint32_t)q.mn << 16) |
-               ((BQ >> 3) << 17) | ((BP >> 4) << 24);
-    const uint64_t tiles = (uint64_t)pr.tiles_p * ((e.rows + BQ - 1) / BQ);
+    pr.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)t.p.mn << 15) | ((uint32_t)t.q.mn << 16) |
+               ((tile_q >> 3) << 17) | ((tile_p >> 4) << 24);
+    return pr;
+}
+template <bool HALF, int COUNT>
+static Products<COUNT> describe_all(const Task* tasks, uint32_t tile_p, uint32_t tile_q, uint32_t box_q) {
+    Products<COUNT> ps;
+    uint64_t tiles = 0;
+    for (int i = 0; i < COUNT; ++i) {
+        ps.of[i] = describe<HALF>(tasks[i], tile_p, tile_q, box_q);
+        tiles += (uint64_t)ps.of[i].tiles_p * ps.of[i].tiles_q;
+    }
+    if (tiles >= (1ull << 28)) throw Error(OZTT_EINVAL, "linear: problem too large");
+    ps.tiles0 = ps.of[0].tiles_p * ps.of[0].tiles_q;
+    ps.tiles = (uint32_t)tiles;
+    return ps;
+}
+
+template <bool HALF, int COUNT, int BQ, int STAGES, int CTAS>
+static void launch_tiles(const Task* tasks, cudaStream_t st) {
+    constexpr uint32_t SMEM = STAGES * (P_BYTES + BQ * BK * 2) + 256 + 1024;
+    static std::atomic<uint64_t> allowed{0};
+    auto* kernel = product_kernel<HALF, COUNT, BQ, STAGES, CTAS>;
+    allow_smem(kernel, SMEM, allowed);
+    const Products<COUNT> ps = describe_all<HALF, COUNT>(tasks, BP, BQ, BQ);
     // With few tiles the reduction is shared by up to 8 CTAs, as long as the CTAs are resident at once and each
     // keeps at least four blocks of it.
+    const uint32_t shortest = std::min(ps.of[0].num_kb, ps.of[COUNT - 1].num_kb);
     uint32_t split = 1;
-    while (split < MAX_SPLIT && tiles * split * 2 <= 148 * CTAS && pr.num_kb / (split * 2) >= 4) split *= 2;
-    if (tiles * split >= (1ull << 31)) throw Error(OZTT_EINVAL, "linear: problem too large");
-    const CUtensorMap tp = operand_map(p, HALF, BP), tq = operand_map(q, HALF, BQ);
-    OZTT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * split), 1, 1);
-    cfg.blockDim = dim3(THREADS, 1, 1);
-    cfg.dynamicSmemBytes = SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = split;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    OZTT_CUDA(cudaLaunchKernelEx(&cfg, kernel, tp, tq, pr, e, error_word()));
+    while (split < MAX_SPLIT && ps.tiles * split * 2 <= 148 * CTAS && shortest / (split * 2) >= 4) split *= 2;
+    launch(kernel, dim3(ps.tiles * split), THREADS, SMEM, dim3(split), st, ps, error_word());
 }
 
-template <bool HALF, int BQ>
-static void launch_pair(const Operand& p, const Operand& q, const Epilogue& e, cudaStream_t st) {
+template <bool HALF, int COUNT, int BQ>
+static void launch_pairs(const Task* tasks, cudaStream_t st) {
     constexpr uint32_t SMEM = PAIR_STAGES_BYTES + FINISHERS * PATCH_BYTES + 256 + 1024;
-    auto* kernel = pair_product_kernel<HALF, BQ>;
-    Product pr;
-    pr.tiles_p = (uint32_t)((e.cols + 2 * BP - 1) / (2 * BP));
-    pr.num_kb = (uint32_t)((p.red + BK - 1) / BK);
-    pr.p_mn = p.mn;
-    pr.q_mn = q.mn;
-    const uint32_t type = HALF ? 0u : 1u;
-    pr.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)p.mn << 15) | ((uint32_t)q.mn << 16) |
-               ((BQ >> 3) << 17) | (((2 * BP) >> 4) << 24);
-    const uint64_t tiles_q = (e.rows + BQ - 1) / BQ, tiles = pr.tiles_p * tiles_q;
-    if (tiles >= (1ull << 31)) throw Error(OZTT_EINVAL, "linear: problem too large");
-    const CUtensorMap tp = operand_map(p, HALF, BP), tq = operand_map(q, HALF, BQ / 2);
-    OZTT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
-    const unsigned grid = 2u * (unsigned)std::min<uint64_t>(tiles, 74);
-    kernel<<<grid, PAIR_THREADS, SMEM, st>>>(tp, tq, pr, (uint32_t)tiles_q, e, error_word());
-    OZTT_CUDA(cudaGetLastError());
+    static std::atomic<uint64_t> allowed{0};
+    auto* kernel = pair_product_kernel<HALF, COUNT, BQ>;
+    allow_smem(kernel, SMEM, allowed);
+    const Products<COUNT> ps = describe_all<HALF, COUNT>(tasks, 2 * BP, BQ, BQ / 2);
+    launch(kernel, dim3(2 * std::min<uint32_t>(ps.tiles, 74)), PAIR_THREADS, SMEM, dim3(0), st, ps, error_word());
 }
 
-// out = epilogue(Q P^T): p the operand of the output's columns, q of its rows.
+template <bool HALF, int M>
+static void launch_few(const Task& t, bool vec, cudaStream_t st) {
+    auto* kernel = vec ? few_rows_kernel<HALF, M, true> : few_rows_kernel<HALF, M, false>;
+    const uint64_t blocks = (t.e.cols + FEW_COLS - 1) / FEW_COLS;
+    // enough warps to keep the memory busy (16 on every SM), as long as each has a few accesses
+    uint32_t warps = 1;
+    while (warps < 8 && blocks * warps < 148 * 16 && t.p.red / (warps * 2) >= 512) warps *= 2;
+    launch(kernel, dim3((unsigned)blocks), warps * 32, 0, dim3(0), st, static_cast<const uint16_t*>(t.p.p), t.p.rs,
+           static_cast<const uint16_t*>(t.q.p), t.q.rs, (uint32_t)t.p.red, t.e);
+}
+
+// The products of one call, out = epilogue(Q P^T): p the operand of the output's columns, q of its rows.
 template <bool HALF>
-static void product(Operand p, Operand q, Epilogue e, cudaStream_t st) {
-    if (e.rows == 0 || e.cols == 0) return;
-    if (e.rows >= (1ull << 31) || e.cols >= (1ull << 31) || p.red >= (1ull << 31))
-        throw Error(OZTT_EINVAL, "linear: dimensions must be below 2^31");
-    DevBuf bp(st), bq(st);
-    if (p.red) {
-        settle(p, true, bp, st);
-        settle(q, e.rows > 32, bq, st);
-    } else {  // nothing is read: any valid address and stride for the tensor maps
-        bp.alloc(256);
-        p.p = q.p = bp.p;
-        p.rs = q.rs = 8;
-        p.ks = q.ks = 1;
-        p.rows = q.rows = 1;
-    }
-    const auto takes = [&](int n) {
-        const auto fits = [n](const View& v) {
-            return !v.p || (v.cs == 1 && v.rs % n == 0 && reinterpret_cast<uintptr_t>(v.p) % (2 * n) == 0);
+static void products(Task* tasks, int count, cudaStream_t st) {
+    std::deque<DevBuf> packed;
+    uint64_t rows = 0, pair_tiles = 0;
+    int live = 0;
+    for (int i = 0; i < count; ++i) {
+        Task t = tasks[i];
+        Epilogue& e = t.e;
+        if (e.rows == 0 || e.cols == 0) continue;
+        if (e.rows >= (1ull << 31) || e.cols >= (1ull << 31) || t.p.red >= (1ull << 31))
+            throw Error(OZTT_EINVAL, "linear: dimensions must be below 2^31");
+        const auto takes = [&](int n) {
+            const auto fits = [n](const View& v) {
+                return !v.p || (v.cs == 1 && v.rs % n == 0 && reinterpret_cast<uintptr_t>(v.p) % (2 * n) == 0);
+            };
+            return fits(e.out) && fits(e.pre) && fits(e.res);
         };
-        return fits(e.out) && fits(e.pre) && fits(e.res);
-    };
-    e.vec = takes(8) ? 8 : takes(4) ? 4 : 1;
-    if (p.red && e.rows > 128 && ((e.rows + 255) / 256) * ((e.cols + 255) / 256) >= 37)
-        launch_pair<HALF, 256>(p, q, e, st);
-    else if (e.rows <= 16)
-        launch_tile<HALF, 16, 6, 2>(p, q, e, st);
-    else if (e.rows <= 32)
-        launch_tile<HALF, 32, 5, 2>(p, q, e, st);
-    else if (e.rows <= 64)
-        launch_tile<HALF, 64, 4, 2>(p, q, e, st);
+        e.vec = takes(8) ? 8 : takes(4) ? 4 : 1;
+        rows = std::max(rows, e.rows);
+        pair_tiles += ((e.rows + 255) / 256) * ((e.cols + 255) / 256);
+        tasks[live++] = t;
+    }
+    if (!live) return;
+    if (live == 2 && std::min(tasks[0].e.rows, tasks[1].e.rows) <= 64) {  // too unlike for tiles of one size
+        products<HALF>(tasks, 1, st);
+        products<HALF>(tasks + 1, 1, st);
+        return;
+    }
+    if (live == 1 && rows <= 4 && tasks[0].p.red && tasks[0].p.ks == 1 && tasks[0].q.ks == 1) {
+        const Task& t = tasks[0];
+        const bool vec = aligned16(t.p.p) && aligned16(t.q.p) && t.p.rs % 8 == 0 && (rows == 1 || t.q.rs % 8 == 0) &&
+                         t.p.red % 8 == 0;
+        const auto run = rows == 1 ? launch_few<HALF, 1> : rows == 2 ? launch_few<HALF, 2> : rows == 3 ? launch_few<HALF, 3> : launch_few<HALF, 4>;
+        return run(t, vec, st);
+    }
+    for (int i = 0; i < live; ++i) {
+        Task& t = tasks[i];
+        if (t.p.red) {
+            packed.emplace_back(st);
+            settle(t.p, true, packed.back(), st);
+            packed.emplace_back(st);
+            settle(t.q, rows > 32, packed.back(), st);
+        } else {  // nothing is read: any valid address and stride for the tensor maps
+            t.p.p = t.q.p = packed.emplace_back(st, 256).p;
+            t.p.rs = t.q.rs = 8;
+            t.p.ks = t.q.ks = 1;
+            t.p.rows = t.q.rows = 1;
+        }
+    }
+    const bool empty = tasks[0].p.red == 0 || tasks[live - 1].p.red == 0;
+    if (!empty && rows > 128 && pair_tiles >= 37)
+        live == 2 ? launch_pairs<HALF, 2, 256>(tasks, st) : launch_pairs<HALF, 1, 256>(tasks, st);
+    else if (rows <= 16)
+        launch_tiles<HALF, 1, 16, 6, 2>(tasks, st);
+    else if (rows <= 32)
+        launch_tiles<HALF, 1, 32, 5, 2>(tasks, st);
+    else if (rows <= 64)
+        launch_tiles<HALF, 1, 64, 4, 2>(tasks, st);
     else
-        launch_tile<HALF, 128, 3, 2>(p, q, e, st);
+        live == 2 ? launch_tiles<HALF, 2, 128, 3, 2>(tasks, st) : launch_tiles<HALF, 1, 128, 3, 2>(tasks, st);
+}
+
+template <bool HALF>
+static auto dz_variant(bool vec, int act) {
+    switch (act) {
+#define OZTT_CASE(A) \
+    case A: return vec ? dz_kernel<HALF, true, A> : dz_kernel<HALF, false, A>
+        OZTT_CASE(OZTT_ACT_RELU);
+        OZTT_CASE(OZTT_ACT_GELU);
+        OZTT_CASE(OZTT_ACT_GELU_TANH);
+        OZTT_CASE(OZTT_ACT_SILU);
+#undef OZTT_CASE
+        default: return vec ? dz_kernel<HALF, true, OZTT_ACT_NONE> : dz_kernel<HALF, false, OZTT_ACT_NONE>;
+    }
 }
 
 static View view(const oztt_view& v) { return {v.data, v.row_stride, v.col_stride}; }
@@ -1059,8 +1328,8 @@ static void forward(int device, const oztt_linear& a, cudaStream_t st) {
     e.bias = a.bias.data;
     e.bias_stride = a.bias.col_stride;
     e.act = a.activation;
-    product<HALF>({a.w.data, a.n, a.k, a.w.row_stride, a.w.col_stride}, {a.x.data, a.m, a.k, a.x.row_stride, a.x.col_stride},
-            e, st);
+    Task t{{a.w.data, a.n, a.k, a.w.row_stride, a.w.col_stride}, {a.x.data, a.m, a.k, a.x.row_stride, a.x.col_stride}, e};
+    products<HALF>(&t, 1, st);
 }
 
 template <bool HALF>
@@ -1078,49 +1347,50 @@ static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
     check_earlier_calls();
     View dz = view(a.dy);
     DevBuf dz_buf(st), sums(st);
-    const bool products = (a.dx.data && a.m && a.k) || (a.dw.data && a.n && a.k);
-    // enough blocks to spread over the device, at least 8 rows each and at most 512
-    const uint64_t strips = (a.n + DZ_COLS - 1) / DZ_COLS;
-    const uint32_t span = (uint32_t)std::min<uint64_t>(512, round_up(std::max<uint64_t>(1, a.m * strips / (148 * 16)), 8));
-    const uint64_t blocks = (a.m + span - 1) / span;
-    if (strips >= (1ull << 31)) throw Error(OZTT_EINVAL, "linear_backward: problem too large");
-    if (a.db.data && mn) sums.alloc(blocks * a.n * 4);
-    if (mn && ((act && products) || a.db.data)) {
-        const uint64_t ld = round_up(a.n, 8);
-        const bool store = act && products;
+    const bool has_products = (a.dx.data && a.m && a.k) || (a.dw.data && a.n && a.k);
+    if (mn && ((act && has_products) || a.db.data)) {
+        // clusters of up to 8 blocks, one below the other, as many as spread over the device; at least 32 rows a block
+        const uint64_t ld = round_up(a.n, 8), strips = (a.n + DZ_COLS - 1) / DZ_COLS, most = (a.m + DZ_ROWS - 1) / DZ_ROWS;
+        uint32_t cluster = 1;
+        while (cluster < DZ_CLUSTER && cluster * 2 <= most) cluster *= 2;
+        const uint64_t clusters = std::max<uint64_t>(1, std::min(most / cluster, (148 * 4) / (strips * cluster)));
+        const uint64_t span = round_up((a.m + clusters * cluster - 1) / (clusters * cluster), DZ_ROWS);
+        const bool store = act && has_products;
         if (store) dz_buf.alloc(a.m * ld * 2);
+        if (a.db.data && clusters > 1) sums.alloc(clusters * a.n * 4);
         const auto fits = [](const View& v) { return !v.p || (v.cs == 1 && v.rs % 8 == 0 && aligned16(v.p)); };
+        auto* db = static_cast<uint16_t*>(a.db.data);
         const View z = act ? view(a.pre) : View{};
-        auto* kernel = fits(dz) && fits(z) ? dz_kernel<HALF, true> : dz_kernel<HALF, false>;
-        for (uint64_t b0 = 0; b0 < blocks; b0 += 65535) {  // the grid's limit of block rows
-            const uint64_t nb = std::min<uint64_t>(65535, blocks - b0), i0 = b0 * span;
-            const auto below = [&](View v) { return View{v.p ? static_cast<uint16_t*>(v.p) + (int64_t)i0 * v.rs : nullptr, v.rs, v.cs}; };
-            kernel<<<dim3((unsigned)strips, (unsigned)nb), DZ_WARPS * 32, 0, st>>>(
-                below(dz), below(z), a.m - i0, a.n, span, a.activation, store ? dz_buf.as<uint16_t>() + i0 * ld : nullptr,
-                ld, a.db.data ? sums.as<float>() + b0 * a.n : nullptr);
-            OZTT_CUDA(cudaGetLastError());
-        }
+        if (strips >= (1ull << 31)) throw Error(OZTT_EINVAL, "linear_backward: problem too large");
+        launch(dz_variant<HALF>(fits(dz) && fits(z) && a.n % 8 == 0, a.activation),
+               dim3((unsigned)strips, (unsigned)(clusters * cluster)), 256, 0, dim3(1, cluster, 1), st, dz, z, a.m, a.n,
+               span, store ? dz_buf.as<uint16_t>() : nullptr, ld, clusters > 1 ? sums.as<float>() : nullptr,
+               clusters > 1 ? nullptr : db, a.db.col_stride);
+        if (a.db.data && clusters > 1)
+            launch(db_kernel<HALF>, dim3((unsigned)((a.n + 31) / 32)), 256, 0, dim3(0), st, sums.as<float>(), clusters, a.n, db,
+                   a.db.col_stride);
         if (store) dz = {dz_buf.p, (int64_t)ld, 1};
+    } else if (a.db.data && a.n) {  // no rows: zeros
+        launch(db_kernel<HALF>, dim3((unsigned)((a.n + 31) / 32)), 256, 0, dim3(0), st, static_cast<const float*>(nullptr),
+               uint64_t{0}, a.n, static_cast<uint16_t*>(a.db.data), a.db.col_stride);
     }
-    if (a.db.data && a.n) {
-        db_kernel<HALF><<<(unsigned)((a.n + 31) / 32), 256, 0, st>>>(sums.as<float>(), a.m ? blocks : 0, a.n,
-                                                                    static_cast<uint16_t*>(a.db.data), a.db.col_stride);
-        OZTT_CUDA(cudaGetLastError());
-    }
+    Task tasks[2];
+    int count = 0;
     Epilogue e{};
     e.act = OZTT_ACT_NONE;
     if (a.dx.data) {  // dx[i][t] = sum_n dz[i][n] w[n][t]
         e.rows = a.m;
         e.cols = a.k;
         e.out = view(a.dx);
-        product<HALF>({a.w.data, a.k, a.n, a.w.col_stride, a.w.row_stride}, {dz.p, a.m, a.n, dz.rs, dz.cs}, e, st);
+        tasks[count++] = {{a.w.data, a.k, a.n, a.w.col_stride, a.w.row_stride}, {dz.p, a.m, a.n, dz.rs, dz.cs}, e};
     }
     if (a.dw.data) {  // dw[n][t] = sum_i dz[i][n] x[i][t]
         e.rows = a.n;
         e.cols = a.k;
         e.out = view(a.dw);
-        product<HALF>({a.x.data, a.k, a.m, a.x.col_stride, a.x.row_stride}, {dz.p, a.n, a.m, dz.cs, dz.rs}, e, st);
+        tasks[count++] = {{a.x.data, a.k, a.m, a.x.col_stride, a.x.row_stride}, {dz.p, a.n, a.m, dz.cs, dz.rs}, e};
     }
+    products<HALF>(tasks, count, st);
 }
 
 }  // namespace layer
