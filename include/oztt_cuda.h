@@ -495,7 +495,7 @@ typedef struct oztt_adamw_tensor {
 
 typedef struct oztt_adamw_moments {
     int32_t bits; /* 8 or 32 */
-    void *m, *v;  /* 16-byte aligned */
+    void *m, *v;  /* 32-byte aligned */
     uint8_t *m_exp, *v_exp; /* with 8 bits */
 } oztt_adamw_moments;
 

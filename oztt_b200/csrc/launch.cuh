@@ -1,0 +1,71 @@
+// SPDX-License-Identifier: Apache-2.0
+// What the asynchronous calls share: the device of a call, and launches that overlap.
+#pragma once
+#include <atomic>
+
+#include "runtime.cuh"
+
+namespace oztt {
+
+// Makes `device` current for one call.
+struct DeviceScope {
+    int before = 0;
+    bool changed = false;
+    explicit DeviceScope(int device) {
+        if (device < 0) throw Error(OZTT_EINVAL, "device_id must be nonnegative");
+        OZTT_CUDA(cudaGetDevice(&before));
+        if (before != device) {
+            OZTT_CUDA(cudaSetDevice(device));
+            changed = true;
+        }
+        static std::atomic<uint64_t> opened{0};
+        if (device < 64 && !(opened.load() >> device & 1)) {
+            open_device(device);
+            opened.fetch_or(1ull << device);
+        }
+    }
+    ~DeviceScope() {
+        if (changed) cudaSetDevice(before);
+    }
+};
+
+// Lets the next kernel of the stream start while this one ends, and waits for the one before, which must be over
+// before anything in memory is read or written (both do nothing where the launch did not ask for the overlap).
+__device__ __forceinline__ void overlap_launches() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Launches a kernel so that it may start while the kernel before it on the stream ends (overlap_launches), its
+// blocks in clusters of `cluster` (as the kernel says where that is {0}).
+template <class... Params, class... Args>
+inline void launch_overlapped(void (*kernel)(Params...), dim3 grid, uint32_t threads, uint32_t smem, dim3 cluster,
+                   cudaStream_t st, Args&&... args) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster.x;
+    attr[1].val.clusterDim.y = cluster.y;
+    attr[1].val.clusterDim.z = cluster.z;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster.x ? 2 : 1;
+    OZTT_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+}
+
+// Allows a kernel its dynamic shared memory, once on each device.
+template <class Kernel>
+inline void allow_smem(Kernel* kernel, uint32_t bytes, std::atomic<uint64_t>& allowed) {
+    int device = 0;
+    OZTT_CUDA(cudaGetDevice(&device));
+    if (device < 64 && (allowed.load() >> device & 1)) return;
+    OZTT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (device < 64) allowed.fetch_or(1ull << device);
+}
+
+}  // namespace oztt

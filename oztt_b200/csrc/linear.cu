@@ -23,7 +23,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "device_scope.cuh"
+#include "launch.cuh"
 #include "runtime.cuh"
 #include "tensor_core.cuh"
 
@@ -219,13 +219,6 @@ struct Products {
         return of[COUNT - 1];
     }
 };
-
-// Lets the next kernel of the stream start while this one ends, and waits for the one before, which must be over
-// before anything in memory is read or written (both do nothing where the launch did not ask for the overlap).
-__device__ __forceinline__ void overlap_launches() {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-}
 
 __device__ __forceinline__ void tma_load_2d(const CUtensorMap* map, uint32_t dst, uint64_t* bar, int32_t c0,
                                             int32_t c1) {
@@ -914,25 +907,30 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint16_t* __restrict__ 
     }
 }
 
-// dz = dy * act'(z) into dz (rows ld apart; may be null), and the sums of its columns in 32 bits. A block takes 64
-// columns (a lane 8 neighbouring ones by 16-byte accesses with VEC, else 8 that are 8 apart) by `span` rows, 32 at
-// a time and twice as many in flight; the blocks of a cluster lie below one another and join their sums, always
-// in the same order, through distributed shared memory: into db where one cluster covers all rows, else into
-// partial[cluster][n] for db_kernel. (db and partial may be null.)
-constexpr uint32_t DZ_COLS = 64, DZ_ROWS = 32, DZ_AHEAD = 2, DZ_CLUSTER = 8;
+// dz = dy * act'(z) into dz (rows ld apart; may be null), and the sums of its columns in 32 bits. A block takes 128
+// columns (a lane 8 neighbouring ones by 16-byte accesses with VEC, else 8 that are 16 apart) by `span` rows, 16 at a
+// time; the blocks of a cluster lie below one another and join their sums, always in the same order, through
+// distributed shared memory: into db where one cluster covers all rows, else into partial[cluster][n] for db_kernel.
+// (db and partial may be null.) Bound by memory, which many warps with few accesses each keep busier than few with
+// many: 8192 x 16384 BF16, one read for db alone: 42 us with 8 blocks on an SM and one row ahead, 61 us with 2 and
+// four (41 at the rate of a copy); two reads with gelu_tanh: 99 us with 4 blocks and two rows ahead, 157 with 2 and
+// four (82); strips of 64 columns take 6 % longer with RELU.
+constexpr uint32_t DZ_COLS = 128, DZ_ROWS = 16, DZ_CLUSTER = 8;
+constexpr uint32_t DZ_LANES = DZ_COLS / 8;
 template <bool HALF, bool VEC, int ACT>
-__global__ void __launch_bounds__(256, 3)
+__global__ void __launch_bounds__(256, !VEC ? 3 : ACT == OZTT_ACT_NONE ? 8 : 4)
     dz_kernel(View dy, View z, uint64_t m, uint64_t n, uint64_t span, uint16_t* __restrict__ dz, uint64_t ld,
               float* __restrict__ partial, uint16_t* __restrict__ db, int64_t db_stride) {
+    constexpr uint32_t DZ_AHEAD = ACT == OZTT_ACT_NONE ? 1 : 2;
     __shared__ float sums[DZ_ROWS][DZ_COLS];
     __shared__ float block_sums[DZ_COLS];
-    const uint32_t r = threadIdx.x >> 3, l = threadIdx.x & 7;
+    const uint32_t r = threadIdx.x / DZ_LANES, l = threadIdx.x % DZ_LANES;
     const uint32_t l0 = VEC ? l * 8 : l;
-    constexpr uint32_t DJ = VEC ? 1 : 8;
+    constexpr uint32_t DJ = VEC ? 1 : DZ_LANES;
     const uint64_t j0 = blockIdx.x * (uint64_t)DZ_COLS + l0;
     const uint64_t i0 = min(blockIdx.y * span, m) + r, i1 = min((blockIdx.y + 1) * span, m);
     // the columns that exist: with VEC (n a multiple of 8) all or none
-    const uint32_t cols = j0 >= n ? 0 : VEC ? 8 : (uint32_t)min((n - j0 + 7) / 8, (uint64_t)8);
+    const uint32_t cols = j0 >= n ? 0 : VEC ? 8 : (uint32_t)min((n - j0 + DJ - 1) / DJ, (uint64_t)8);
     overlap_launches();
     f32x2 sum[4] = {};
     if (cols && i0 < i1) {
@@ -1069,36 +1067,6 @@ struct Operand {
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Launches a kernel so that it may start while the kernel before it on the stream ends (overlap_launches), its
-// blocks in clusters of `cluster` (as the kernel says where that is {0}).
-template <class... Params, class... Args>
-static void launch(void (*kernel)(Params...), dim3 grid, uint32_t threads, uint32_t smem, dim3 cluster,
-                   cudaStream_t st, Args&&... args) {
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cluster.x;
-    attr[1].val.clusterDim.y = cluster.y;
-    attr[1].val.clusterDim.z = cluster.z;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads, 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster.x ? 2 : 1;
-    OZTT_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
-}
-template <class Kernel>
-static void allow_smem(Kernel* kernel, uint32_t bytes, std::atomic<uint64_t>& allowed) {
-    int device = 0;
-    OZTT_CUDA(cudaGetDevice(&device));
-    if (device < 64 && (allowed.load() >> device & 1)) return;
-    OZTT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    if (device < 64) allowed.fetch_or(1ull << device);
-}
-
 // The operand as the tensor copies can read it: as it lies (K-major, or MN-major where allowed), or packed.
 static void settle(Operand& o, bool allow_mn, DevBuf& buf, cudaStream_t st) {
     if (o.red == 1) o.ks = 1;  // a stride that no element uses
@@ -1115,7 +1083,7 @@ static void settle(Operand& o, bool allow_mn, DevBuf& buf, cudaStream_t st) {
     const uint64_t outer = mn ? o.red : o.rows, inner = mn ? o.rows : o.red, ld = round_up(inner, 8);
     buf.alloc(outer * ld * 2);
     const unsigned grid = (unsigned)std::min<uint64_t>((outer * (ld / 8) + 255) / 256, 148 * 16);
-    launch(pack_kernel, dim3(grid), 256, 0, dim3(0), st, static_cast<const uint16_t*>(o.p), mn ? o.ks : o.rs,
+    launch_overlapped(pack_kernel, dim3(grid), 256, 0, dim3(0), st, static_cast<const uint16_t*>(o.p), mn ? o.ks : o.rs,
            mn ? o.rs : o.ks, outer, inner, buf.as<uint16_t>(), ld);
     o.p = buf.p;
     o.mn = mn;
@@ -1186,7 +1154,7 @@ static void launch_tiles(const Task* tasks, cudaStream_t st) {
     const uint32_t shortest = std::min(ps.of[0].num_kb, ps.of[COUNT - 1].num_kb);
     uint32_t split = 1;
     while (split < MAX_SPLIT && ps.tiles * split * 2 <= 148 * CTAS && shortest / (split * 2) >= 4) split *= 2;
-    launch(kernel, dim3(ps.tiles * split), THREADS, SMEM, dim3(split), st, ps, error_word());
+    launch_overlapped(kernel, dim3(ps.tiles * split), THREADS, SMEM, dim3(split), st, ps, error_word());
 }
 
 template <bool HALF, int COUNT, int BQ>
@@ -1196,7 +1164,7 @@ static void launch_pairs(const Task* tasks, cudaStream_t st) {
     auto* kernel = pair_product_kernel<HALF, COUNT, BQ>;
     allow_smem(kernel, SMEM, allowed);
     const Products<COUNT> ps = describe_all<HALF, COUNT>(tasks, 2 * BP, BQ, BQ / 2);
-    launch(kernel, dim3(2 * std::min<uint32_t>(ps.tiles, 74)), PAIR_THREADS, SMEM, dim3(0), st, ps, error_word());
+    launch_overlapped(kernel, dim3(2 * std::min<uint32_t>(ps.tiles, 74)), PAIR_THREADS, SMEM, dim3(0), st, ps, error_word());
 }
 
 template <bool HALF, int M>
@@ -1206,7 +1174,7 @@ static void launch_few(const Task& t, bool vec, cudaStream_t st) {
     // enough warps to keep the memory busy (16 on every SM), as long as each has a few accesses
     uint32_t warps = 1;
     while (warps < 8 && blocks * warps < 148 * 16 && t.p.red / (warps * 2) >= 512) warps *= 2;
-    launch(kernel, dim3((unsigned)blocks), warps * 32, 0, dim3(0), st, static_cast<const uint16_t*>(t.p.p), t.p.rs,
+    launch_overlapped(kernel, dim3((unsigned)blocks), warps * 32, 0, dim3(0), st, static_cast<const uint16_t*>(t.p.p), t.p.rs,
            static_cast<const uint16_t*>(t.q.p), t.q.rs, (uint32_t)t.p.red, t.e);
 }
 
@@ -1349,11 +1317,13 @@ static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
     DevBuf dz_buf(st), sums(st);
     const bool has_products = (a.dx.data && a.m && a.k) || (a.dw.data && a.n && a.k);
     if (mn && ((act && has_products) || a.db.data)) {
-        // clusters of up to 8 blocks, one below the other, as many as spread over the device; at least 32 rows a block
+        // clusters of up to 8 blocks, one below the other, as many as spread over the device; at least 16 rows a block
         const uint64_t ld = round_up(a.n, 8), strips = (a.n + DZ_COLS - 1) / DZ_COLS, most = (a.m + DZ_ROWS - 1) / DZ_ROWS;
         uint32_t cluster = 1;
         while (cluster < DZ_CLUSTER && cluster * 2 <= most) cluster *= 2;
-        const uint64_t clusters = std::max<uint64_t>(1, std::min(most / cluster, (148 * 4) / (strips * cluster)));
+        // (up to 128 rows a block need no second cluster, nor the launch that joins the clusters' sums)
+        const uint64_t clusters =
+            most <= 8 * cluster ? 1 : std::max<uint64_t>(1, std::min(most / cluster, (148 * 4) / (strips * cluster)));
         const uint64_t span = round_up((a.m + clusters * cluster - 1) / (clusters * cluster), DZ_ROWS);
         const bool store = act && has_products;
         if (store) dz_buf.alloc(a.m * ld * 2);
@@ -1362,16 +1332,16 @@ static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
         auto* db = static_cast<uint16_t*>(a.db.data);
         const View z = act ? view(a.pre) : View{};
         if (strips >= (1ull << 31)) throw Error(OZTT_EINVAL, "linear_backward: problem too large");
-        launch(dz_variant<HALF>(fits(dz) && fits(z) && a.n % 8 == 0, a.activation),
+        launch_overlapped(dz_variant<HALF>(fits(dz) && fits(z) && a.n % 8 == 0, a.activation),
                dim3((unsigned)strips, (unsigned)(clusters * cluster)), 256, 0, dim3(1, cluster, 1), st, dz, z, a.m, a.n,
                span, store ? dz_buf.as<uint16_t>() : nullptr, ld, clusters > 1 ? sums.as<float>() : nullptr,
                clusters > 1 ? nullptr : db, a.db.col_stride);
         if (a.db.data && clusters > 1)
-            launch(db_kernel<HALF>, dim3((unsigned)((a.n + 31) / 32)), 256, 0, dim3(0), st, sums.as<float>(), clusters, a.n, db,
+            launch_overlapped(db_kernel<HALF>, dim3((unsigned)((a.n + 31) / 32)), 256, 0, dim3(0), st, sums.as<float>(), clusters, a.n, db,
                    a.db.col_stride);
         if (store) dz = {dz_buf.p, (int64_t)ld, 1};
     } else if (a.db.data && a.n) {  // no rows: zeros
-        launch(db_kernel<HALF>, dim3((unsigned)((a.n + 31) / 32)), 256, 0, dim3(0), st, static_cast<const float*>(nullptr),
+        launch_overlapped(db_kernel<HALF>, dim3((unsigned)((a.n + 31) / 32)), 256, 0, dim3(0), st, static_cast<const float*>(nullptr),
                uint64_t{0}, a.n, static_cast<uint16_t*>(a.db.data), a.db.col_stride);
     }
     Task tasks[2];
