@@ -270,6 +270,16 @@ def __getattr__(name: str):
     raise AttributeError(name)
 
 
+def _binding():
+    """The binding of the calls on torch's tensors (``_torch.so``)."""
+    try:
+        from . import _torch
+    except ImportError as e:
+        raise ImportError(f"oztt_b200/_torch.so is not built for this torch and Python ({e}); run "
+                          "`python -m oztt_b200.build` (or __graft_entry__.build()) first") from e
+    return _torch
+
+
 def _raise(code: int, msg: bytes | str) -> None:
     text = msg.decode(errors="replace") if isinstance(msg, bytes) else msg
     if code == EINVAL:

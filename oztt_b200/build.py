@@ -3,6 +3,7 @@
 Produces
   oztt_b200/liboztt.so            the CUDA kernels for sm_100a, the planner, the C ABI
                                   (include/oztt_cuda.h) and the C++ API (include/ozTTgemm/ozTTgemm.hpp)
+  oztt_b200/_torch.so             csrc/torch_binding.cpp: the calls on torch's CUDA tensors over the C ABI
   oztt_b200/_build/gemm_example   examples/gemm.cpp linked against it
   oztt_b200/_build/correctness    tests/cpp/correctness.cpp linked against it
 Object files go to oztt_b200/_build/. Nothing is installed outside the repository; the built files
@@ -24,6 +25,7 @@ PKG = ROOT / "oztt_b200"
 CSRC = PKG / "csrc"
 OUT = PKG / "_build"
 LIB = PKG / "liboztt.so"
+BINDING = PKG / "_torch.so"
 
 NVCC = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
 # The system compiler: the environment's CXX may name a toolchain without OpenMP support files.
@@ -83,6 +85,26 @@ def build_library(force: bool = False) -> Path:
     return LIB
 
 
+def build_torch_binding(force: bool = False) -> Path:
+    """oztt_b200/_torch.so: the binding of the calls on torch's tensors to the C ABI, for the torch of this
+    interpreter."""
+    import importlib.util
+    import sysconfig
+
+    torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    src = CSRC / "torch_binding.cpp"
+    # built again for another torch or Python
+    stamp, made_for = OUT / "torch_binding.for", f"{torch} {(torch / 'version.py').read_text()} {sys.version}"
+    if force or _stale(BINDING, [src, ROOT / "include" / "oztt_cuda.h"]) or not stamp.exists() or stamp.read_text() != made_for:
+        _run([CXX, "-std=c++17", "-O2", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=1", f"-I{ROOT / 'include'}",
+              f"-I{torch / 'include'}", f"-I{torch / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+              f"-I{sysconfig.get_paths()['include']}", f"-I{CUDA_HOME / 'include'}", str(src), "-o", str(BINDING),
+              f"-L{PKG}", "-loztt", "-Wl,-rpath,$ORIGIN", f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch",
+              "-lc10", "-lc10_cuda"])
+        stamp.write_text(made_for)
+    return BINDING
+
+
 def build_programs(force: bool = False) -> None:
     progs = {
         "gemm_example": ROOT / "examples" / "gemm.cpp",
@@ -118,6 +140,7 @@ def build_oracle() -> None:
 
 def build(force: bool = False) -> None:
     build_library(force)
+    build_torch_binding(force)
     build_programs(force)
     build_oracle()
 

@@ -1,0 +1,293 @@
+// SPDX-License-Identifier: Apache-2.0
+//
+// The calls on torch's CUDA tensors (layers.py, optim.py) over the C ABI: the checks of their arguments, the tensors
+// of their results and the current stream, in C++ because a single token's product takes 7 us on the device and the
+// same steps in Python take as long (a step over 300 tensors: 100 us).
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAStream.h>
+#include <c10/core/GradMode.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cstring>
+#include <sstream>
+#include <stdexcept>
+#include <string>
+
+#include "oztt_cuda.h"
+
+namespace {
+
+// Refusals, raised as ValueError.
+struct Refused : std::runtime_error {
+    using std::runtime_error::runtime_error;
+};
+[[noreturn]] void refuse(const std::string& text) { throw Refused(text); }
+
+std::string text(const at::Tensor& t) {
+    std::ostringstream s;
+    s << '[';
+    for (int64_t i = 0; i < t.dim(); ++i) s << (i ? ", " : "") << t.size(i);
+    s << ']';
+    return s.str();
+}
+
+// Runs f, raising what it throws.
+template <class F>
+PyObject* guarded(F&& f) {
+    try {
+        return f();
+    } catch (const Refused& e) {
+        PyErr_SetString(PyExc_ValueError, e.what());
+    } catch (const c10::OutOfMemoryError& e) {
+        PyErr_SetString(PyExc_MemoryError, e.what_without_backtrace());
+    } catch (const c10::Error& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
+    } catch (const std::bad_alloc&) {
+        PyErr_SetString(PyExc_MemoryError, "host memory exhausted");
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    }
+    return nullptr;
+}
+
+// One call of the C ABI without the interpreter's lock; its codes as layers.py's callers know them.
+template <class F>
+void call(F&& f) {
+    char err[1024];
+    int rc;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = f(err, sizeof err);
+    Py_END_ALLOW_THREADS;
+    if (rc == OZTT_OK) return;
+    if (rc == OZTT_EINVAL) refuse(err);
+    if (rc == OZTT_ENOMEM) throw std::bad_alloc();
+    throw std::runtime_error(err);
+}
+
+const at::Tensor* tensor_or_none(PyObject* o, const char* who, const char* what) {
+    if (o == Py_None) return nullptr;
+    if (!THPVariable_Check(o)) refuse(std::string(who) + ": " + what + " must be a tensor");
+    return &THPVariable_Unpack(o);
+}
+const at::Tensor& tensor(PyObject* o, const char* who, const char* what) {
+    const at::Tensor* t = tensor_or_none(o, who, what);
+    if (!t) refuse(std::string(who) + ": " + what + " is missing");
+    return *t;
+}
+
+int32_t format_of(const at::Tensor& t, const char* who) {
+    if (!t.is_cuda()) refuse(std::string(who) + ": the tensors must be on a CUDA device");
+    if (t.scalar_type() == at::kBFloat16) return OZTT_FMT_BF16;
+    if (t.scalar_type() == at::kHalf) return OZTT_FMT_FP16;
+    refuse(std::string(who) + ": the type must be torch.bfloat16 or torch.float16, not " + c10::toString(t.scalar_type()));
+}
+void same_kind(const at::Tensor& first, const at::Tensor* t, const char* who, const char* what) {
+    if (t && (t->scalar_type() != first.scalar_type() || t->device() != first.device()))
+        refuse(std::string(who) + ": " + what + " must be " + c10::toString(first.scalar_type()) + " on " + first.device().str());
+}
+
+// A matrix, or a vector as one row.
+oztt_view view(const at::Tensor& t) {
+    const bool matrix = t.dim() == 2;
+    return {t.data_ptr(), matrix ? t.stride(0) : 0, t.stride(matrix ? 1 : 0)};
+}
+oztt_view view(const at::Tensor* t) { return t ? view(*t) : oztt_view{nullptr, 0, 0}; }
+
+at::Tensor rows_of(const at::Tensor& t, int64_t rows, int64_t cols) { return t.dim() == 2 ? t : t.reshape({rows, cols}); }
+
+bool wants_gradient(std::initializer_list<const at::Tensor*> all) {
+    if (!c10::GradMode::is_enabled()) return false;
+    for (const at::Tensor* t : all)
+        if (t && t->requires_grad()) return true;
+    return false;
+}
+
+PyObject* wrapped(const at::Tensor& t) {
+    if (t.defined()) return THPVariable_Wrap(t);
+    Py_RETURN_NONE;
+}
+
+bool expect(Py_ssize_t got, Py_ssize_t wanted, const char* who) {
+    if (got == wanted) return true;
+    PyErr_Format(PyExc_TypeError, "%s takes %zd arguments", who, wanted);
+    return false;
+}
+
+// linear(x, weight, bias, residual, activation, save_pre, differentiable) -> (y, pre or None), or None where a
+// gradient is wanted and `differentiable`: the caller records the call then.
+PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    if (!expect(count, 7, "linear")) return nullptr;
+    return guarded([&]() -> PyObject* {
+        constexpr const char* who = "linear";
+        const at::Tensor &x = tensor(args[0], who, "x"), &w = tensor(args[1], who, "weight");
+        const at::Tensor *b = tensor_or_none(args[2], who, "bias"), *r = tensor_or_none(args[3], who, "residual");
+        const bool save_pre = args[5] == Py_True;
+        oztt_linear a{};
+        a.format = format_of(x, who);
+        same_kind(x, &w, who, "weight");
+        same_kind(x, b, who, "bias");
+        same_kind(x, r, who, "residual");
+        a.activation = (int32_t)PyLong_AsLong(args[4]);
+        const int64_t dim = x.dim();
+        if (w.dim() != 2 || !dim || x.size(dim - 1) != w.size(1))
+            refuse("linear: x " + text(x) + " does not match weight " + text(w));
+        const int64_t n = w.size(0), k = w.size(1);
+        if (b && (b->dim() != 1 || b->size(0) != n)) refuse("linear: bias " + text(*b) + " does not match weight " + text(w));
+        int64_t m = 1;
+        bool fits = !r || r->dim() == dim;
+        for (int64_t i = 0; i + 1 < dim; ++i) {
+            m *= x.size(i);
+            fits = fits && (!r || r->size(i) == x.size(i));
+        }
+        if (r && !(fits && r->size(dim - 1) == n))
+            refuse("linear: residual " + text(*r) + " does not match the output of x " + text(x) + " and weight " + text(w));
+        if (args[6] == Py_True && wants_gradient({&x, &w, b, r})) Py_RETURN_NONE;
+        at::NoGradGuard no_grad;
+        const at::Tensor x2 = rows_of(x, m, k);
+        const at::Tensor r2 = r ? rows_of(*r, m, n) : at::Tensor();
+        at::Tensor y = at::empty({m, n}, x.options().requires_grad(false)), pre;
+        if (save_pre) pre = at::empty_like(y);
+        a.m = (uint64_t)m;
+        a.n = (uint64_t)n;
+        a.k = (uint64_t)k;
+        a.x = view(x2);
+        a.w = view(w);
+        a.bias = view(b);
+        if (r) a.residual = view(r2);
+        a.y = view(y);
+        if (save_pre) a.pre = view(pre);
+        const int device = x.get_device();
+        void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+        call([&](char* err, size_t len) { return oztt_linear_forward(device, &a, stream, err, len); });
+        if (dim != 2) {
+            auto shape = x.sizes().vec();
+            shape.back() = n;
+            y = y.view(shape);
+            if (save_pre) pre = pre.view(shape);
+        }
+        return Py_BuildValue("(NN)", wrapped(y), wrapped(pre));
+    });
+}
+
+// linear_backward(dy, x, weight, pre, activation, need_input, need_weight, need_bias) -> (dx, dw, db)
+PyObject* linear_backward(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    if (!expect(count, 8, "linear_backward")) return nullptr;
+    return guarded([&]() -> PyObject* {
+        constexpr const char* who = "linear_backward";
+        const at::Tensor &dy = tensor(args[0], who, "dy"), &x = tensor(args[1], who, "x"), &w = tensor(args[2], who, "weight");
+        const at::Tensor* pre = tensor_or_none(args[3], who, "pre");
+        oztt_linear_grad a{};
+        a.format = format_of(dy, who);
+        same_kind(dy, &x, who, "x");
+        same_kind(dy, &w, who, "weight");
+        same_kind(dy, pre, who, "pre");
+        a.activation = (int32_t)PyLong_AsLong(args[4]);
+        const int64_t dim = x.dim();
+        if (w.dim() != 2 || !dim || x.size(dim - 1) != w.size(1))
+            refuse("linear_backward: x " + text(x) + " does not match weight " + text(w));
+        const int64_t n = w.size(0), k = w.size(1);
+        int64_t m = 1;
+        bool fits = dy.dim() == dim && dy.size(dim - 1) == n;
+        for (int64_t i = 0; i + 1 < dim; ++i) {
+            m *= x.size(i);
+            fits = fits && dy.size(i) == x.size(i);
+        }
+        if (!fits) refuse("linear_backward: dy " + text(dy) + " does not match x " + text(x) + " and weight " + text(w));
+        if (a.activation != OZTT_ACT_NONE && !pre) refuse("linear_backward: the activation needs pre");
+        if (pre && pre->sizes() != dy.sizes())
+            refuse("linear_backward: pre " + text(*pre) + " does not match dy " + text(dy));
+        at::NoGradGuard no_grad;
+        const at::Tensor x2 = rows_of(x, m, k), dy2 = rows_of(dy, m, n), pre2 = pre ? rows_of(*pre, m, n) : at::Tensor();
+        const auto options = dy.options().requires_grad(false);
+        at::Tensor dx, dw, db;
+        if (args[5] == Py_True) dx = at::empty({m, k}, options);
+        if (args[6] == Py_True) dw = at::empty({n, k}, options);
+        if (args[7] == Py_True) db = at::empty({n}, options);
+        a.m = (uint64_t)m;
+        a.n = (uint64_t)n;
+        a.k = (uint64_t)k;
+        a.dy = view(dy2);
+        a.x = view(x2);
+        a.w = view(w);
+        if (pre) a.pre = view(pre2);
+        if (dx.defined()) a.dx = view(dx);
+        if (dw.defined()) a.dw = view(dw);
+        if (db.defined()) a.db = view(db);
+        if (dx.defined() || dw.defined() || db.defined()) {
+            const int device = dy.get_device();
+            void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+            call([&](char* err, size_t len) { return oztt_linear_backward(device, &a, stream, err, len); });
+        }
+        if (dim != 2 && dx.defined()) dx = dx.view(x.sizes());
+        return Py_BuildValue("(NNN)", wrapped(dx), wrapped(dw), wrapped(db));
+    });
+}
+
+int32_t type_of(const at::Tensor& t) {
+    switch (t.scalar_type()) {
+        case at::kBFloat16: return OZTT_TYPE_BF16;
+        case at::kHalf: return OZTT_TYPE_FP16;
+        case at::kFloat: return OZTT_TYPE_FP32;
+        default: return -1;
+    }
+}
+
+// adamw_step(table, grads, grad_scale, moments, hyper, device): table a writable buffer of oztt_adamw_tensor, one for
+// each parameter, whose gradients are filled in here; grads a list or tuple; moments and hyper bytes of
+// oztt_adamw_moments and oztt_adamw_hyper (with grad_scale filled in here).
+PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    if (!expect(count, 6, "adamw_step")) return nullptr;
+    Py_buffer table;
+    if (PyObject_GetBuffer(args[0], &table, PyBUF_WRITABLE) != 0) return nullptr;
+    PyObject* result = guarded([&]() -> PyObject* {
+        auto* t = static_cast<oztt_adamw_tensor*>(table.buf);
+        const Py_ssize_t n = table.len / (Py_ssize_t)sizeof(oztt_adamw_tensor);
+        if (!PyList_Check(args[1]) && !PyTuple_Check(args[1])) refuse("AdamW: grads must be a list or a tuple");
+        if (PySequence_Fast_GET_SIZE(args[1]) != n) refuse("AdamW: grads must be as many as params");
+        PyObject** grads = PySequence_Fast_ITEMS(args[1]);
+        const int device = (int)PyLong_AsLong(args[5]);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            const at::Tensor* g = tensor_or_none(grads[i], "AdamW", "a gradient");
+            t[i].grad = nullptr;
+            if (!g) continue;
+            const int32_t type = type_of(*g);
+            const auto which = [&] { return "AdamW: gradient " + std::to_string(i); };
+            if (type < 0) refuse(which() + " must be BF16, FP16 or FP32");
+            if (!g->is_cuda() || g->get_device() != device) refuse(which() + " must be on the parameters' device");
+            if ((uint64_t)g->numel() != t[i].count) refuse(which() + "'s size is not its parameter's");
+            if (!g->is_contiguous()) refuse(which() + " must be contiguous");
+            t[i].grad = g->data_ptr();
+            t[i].grad_type = type;
+        }
+        oztt_adamw_moments moments;
+        oztt_adamw_hyper hyper;
+        if (PyBytes_GET_SIZE(args[3]) != sizeof moments || PyBytes_GET_SIZE(args[4]) != sizeof hyper)
+            throw std::runtime_error("adamw_step: records of another size");
+        std::memcpy(&moments, PyBytes_AS_STRING(args[3]), sizeof moments);
+        std::memcpy(&hyper, PyBytes_AS_STRING(args[4]), sizeof hyper);
+        if (const at::Tensor* s = tensor_or_none(args[2], "AdamW", "grad_scale")) {
+            if (s->scalar_type() != at::kFloat || !s->is_cuda() || s->get_device() != device || s->numel() != 1)
+                refuse("AdamW: grad_scale must be one FP32 number on the parameters' device");
+            hyper.grad_scale = s->const_data_ptr<float>();
+        }
+        void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+        call([&](char* err, size_t len) { return oztt_adamw_step(device, t, (uint64_t)n, &moments, &hyper, stream, err, len); });
+        Py_RETURN_NONE;
+    });
+    PyBuffer_Release(&table);
+    return result;
+}
+
+PyMethodDef methods[] = {
+    {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear)), METH_FASTCALL, nullptr},
+    {"linear_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear_backward)), METH_FASTCALL, nullptr},
+    {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(adamw_step)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__torch() { return PyModule_Create(&module); }

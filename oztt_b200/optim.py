@@ -4,12 +4,11 @@ C ABI). No counterpart in the reference."""
 from __future__ import annotations
 
 import struct
-from operator import attrgetter
 
 import numpy as np
 import torch
 
-from . import OK, _errbuf, _lib, _raise
+from . import OK, _binding, _errbuf, _lib, _raise
 
 __all__ = ["AdamW"]
 
@@ -22,7 +21,7 @@ _TENSOR = np.dtype([("param", np.uint64), ("grad", np.uint64), ("master", np.uin
 _MOMENTS = struct.Struct("=i4x4Q")
 _HYPER = struct.Struct("=5dQQI4x")
 
-_dtype, _device = attrgetter("dtype"), attrgetter("device")
+_torch = _binding()  # csrc/torch_binding.cpp: the gradients' checks and addresses, the current stream
 
 
 class AdamW:
@@ -88,17 +87,8 @@ class AdamW:
         self._table["count"] = self._counts
         self._table["param_type"] = [_TYPES[p.dtype] for p in params]
         self._grown = [p for p in params if p.requires_grad]
-        self._err = _errbuf()
-
-    def _moments(self) -> bytes:
-        exps = (self.m_exp.data_ptr(), self.v_exp.data_ptr()) if self.state_bits == 8 else (0, 0)
-        return _MOMENTS.pack(self.state_bits, self.m.data_ptr(), self.v.data_ptr(), *exps)
-
-    def _call(self, name: str, *args) -> None:
-        rc = getattr(_lib(), name)(self.device.index, *args, torch._C._cuda_getCurrentRawStream(self.device.index),
-                                   self._err, len(self._err))
-        if rc != OK:
-            _raise(rc, self._err.value)
+        exps = (self.m_exp.data_ptr(), self.v_exp.data_ptr()) if state_bits == 8 else (0, 0)
+        self._record = _MOMENTS.pack(state_bits, self.m.data_ptr(), self.v.data_ptr(), *exps)
 
     def step(self, grads=None, *, grad_scale: torch.Tensor | None = None, lr: float | None = None,
              seed: int | None = None) -> None:
@@ -110,40 +100,12 @@ class AdamW:
         repeats the same step."""
         if grads is None:
             grads = [p.grad for p in self.params]
-        if len(grads) != len(self.params):
-            raise ValueError("AdamW: grads must be as many as params")
-        table = self._table
-        counts, live = self._counts, grads
-        if any(g is None for g in grads):
-            counts = [n for n, g in zip(counts, grads) if g is not None]
-            live = [g for g in grads if g is not None]
-        if live:
-            kinds = set(map(_dtype, live))
-            if not kinds <= _TYPES.keys():
-                raise ValueError("AdamW: gradients must be BF16, FP16 or FP32")
-            if set(map(_device, live)) != {self.device}:
-                raise ValueError(f"AdamW: gradients must be on {self.device}")
-            if list(map(torch.Tensor.numel, live)) != counts:
-                raise ValueError("AdamW: a gradient's size is not its parameter's")
-            if not all(map(torch.Tensor.is_contiguous, live)):
-                raise ValueError("AdamW: gradients must be contiguous")
-            if live is grads:
-                table["grad"] = list(map(torch.Tensor.data_ptr, grads))
-                table["grad_type"] = _TYPES[next(iter(kinds))] if len(kinds) == 1 else [_TYPES[g.dtype] for g in grads]
-            else:
-                table["grad"] = [0 if g is None else g.data_ptr() for g in grads]
-                table["grad_type"] = [0 if g is None else _TYPES[g.dtype] for g in grads]
-        else:
-            table["grad"] = 0
-        if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.device != self.device
-                                       or grad_scale.numel() != 1):
-            raise ValueError(f"AdamW: grad_scale must be one FP32 number on {self.device}")
         t = self.t + 1
         if seed is None:
             seed = self.seed + 0x632BE5AB * t
         hyper = _HYPER.pack(self.lr if lr is None else lr, *self.betas, self.eps, self.weight_decay, t,
-                            0 if grad_scale is None else grad_scale.data_ptr(), seed & 0xFFFFFFFF)
-        self._call("oztt_adamw_step", table.ctypes.data, len(self.params), self._moments(), hyper)
+                            0, seed & 0xFFFFFFFF)
+        _torch.adamw_step(self._table, grads, grad_scale, self._record, hyper, self.device.index)
         self.t = t
         if self._grown:  # saved for a backward pass that has not run, they are no longer what was saved
             torch.autograd.graph.increment_version(self._grown)
@@ -154,7 +116,11 @@ class AdamW:
         if self.state_bits == 32:
             return self.m, self.v
         m, v = (torch.empty(self.blocks * BLOCK, dtype=torch.bfloat16, device=self.device) for _ in range(2))
-        self._call("oztt_adamw_values", self._moments(), self.blocks, m.data_ptr(), v.data_ptr())
+        err = _errbuf()
+        rc = _lib().oztt_adamw_values(self.device.index, self._record, self.blocks, m.data_ptr(), v.data_ptr(),
+                                      torch.cuda.current_stream(self.device).cuda_stream, err, len(err))
+        if rc != OK:
+            _raise(rc, err.value)
         return m, v
 
     def state_dict(self) -> dict:
