@@ -18,7 +18,6 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
-#include <deque>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -886,24 +885,37 @@ __global__ void __launch_bounds__(256)
 
 // ---- passes over memory --------------------------------------------------------------------------
 
-// dst[o][i] = src[o * so + i * si], rows ld apart (ld a multiple of 8, zero beyond `inner`): operands whose base
-// or rows do not start on 16 bytes, which the tensor copies cannot read.
-__global__ void __launch_bounds__(256) pack_kernel(const uint16_t* __restrict__ src, int64_t so, int64_t si,
-                                                   uint64_t outer, uint64_t inner, uint16_t* __restrict__ dst,
-                                                   uint64_t ld) {
-    const uint64_t per_row = ld / 8, count = outer * per_row;
+// Copies of operands whose base or rows do not start on 16 bytes, which the tensor copies cannot read:
+// dst[o][i] = src[o * so + i * si], rows ld apart (a multiple of 8, zero beyond `inner`). Up to 4 in one launch.
+struct Pack {
+    const uint16_t* src;
+    int64_t so, si;
+    uint64_t outer, inner, ld;
+    uint16_t* dst;
+    uint64_t end;  // groups of 8 elements of this copy and those before it
+};
+struct Packs {
+    Pack of[4];
+    uint32_t count;
+};
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs packs) {
     overlap_launches();
-    for (uint64_t t = blockIdx.x * (uint64_t)blockDim.x + threadIdx.x; t < count; t += (uint64_t)gridDim.x * blockDim.x) {
-        const uint64_t o = t / per_row, i = (t - o * per_row) * 8;
+    const uint64_t all = packs.of[packs.count - 1].end;
+    for (uint64_t t = blockIdx.x * (uint64_t)blockDim.x + threadIdx.x; t < all; t += (uint64_t)gridDim.x * blockDim.x) {
+        uint32_t c = 0;
+        while (t >= packs.of[c].end) ++c;
+        const Pack& k = packs.of[c];
+        const uint64_t g = t - (c ? packs.of[c - 1].end : 0), per_row = k.ld / 8;
+        const uint64_t o = (g | per_row) >> 32 ? g / per_row : (uint32_t)g / (uint32_t)per_row, i = (g - o * per_row) * 8;
+        const uint16_t* src = k.src + (int64_t)o * k.so + (int64_t)i * k.si;
         uint32_t w[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const uint64_t i0 = i + 2 * q;
-            const uint32_t lo = i0 < inner ? src[(int64_t)o * so + (int64_t)i0 * si] : 0;
-            const uint32_t hi = i0 + 1 < inner ? src[(int64_t)o * so + (int64_t)(i0 + 1) * si] : 0;
+            const uint32_t lo = i + 2 * q < k.inner ? src[2 * q * k.si] : 0;
+            const uint32_t hi = i + 2 * q + 1 < k.inner ? src[(2 * q + 1) * k.si] : 0;
             w[q] = lo | (hi << 16);
         }
-        *reinterpret_cast<uint4*>(dst + o * ld + i) = make_uint4(w[0], w[1], w[2], w[3]);
+        store_words(k.dst + o * k.ld + i, w);
     }
 }
 
@@ -1063,33 +1075,63 @@ struct Operand {
     uint64_t rows, red;
     int64_t rs, ks;
     bool mn = false;
+    int64_t at = -1;  // where it will lie in the call's scratch memory, if it does
 };
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// The operand as the tensor copies can read it: as it lies (K-major, or MN-major where allowed), or packed.
-static void settle(Operand& o, bool allow_mn, DevBuf& buf, cudaStream_t st) {
-    if (o.red == 1) o.ks = 1;  // a stride that no element uses
-    if (o.rows == 1) o.rs = (int64_t)round_up(o.red, 8);
-    const bool base = aligned16(o.p);
-    if (o.ks == 1 && o.rs % 8 == 0 && o.rs >= (int64_t)o.red && base) return;
-    if (o.red == 1) o.ks = (int64_t)round_up(o.rows, 8);
-    if (allow_mn && o.rs == 1 && o.ks % 8 == 0 && o.ks >= (int64_t)o.rows && base) {
-        o.mn = true;
-        return;
+// One call's scratch memory: laid out first, then allocated at once, and the operands' copies made in one launch.
+struct Scratch {
+    cudaStream_t st;
+    uint64_t bytes = 0;
+    DevBuf buf;
+    Packs packs;
+    uint64_t pack_at[4];
+    explicit Scratch(cudaStream_t s) : st(s), buf(s) { packs.count = 0; }
+    int64_t reserve(uint64_t size) {
+        const uint64_t at = bytes;
+        bytes += round_up(std::max<uint64_t>(size, 1), 256);
+        return (int64_t)at;
     }
-    // packed along the contiguous index, so that the copy reads and writes neighbouring elements
-    const bool mn = allow_mn && o.rs == 1 && o.ks != 1;
-    const uint64_t outer = mn ? o.red : o.rows, inner = mn ? o.rows : o.red, ld = round_up(inner, 8);
-    buf.alloc(outer * ld * 2);
-    const unsigned grid = (unsigned)std::min<uint64_t>((outer * (ld / 8) + 255) / 256, 148 * 16);
-    launch_overlapped(pack_kernel, dim3(grid), 256, 0, dim3(0), st, static_cast<const uint16_t*>(o.p), mn ? o.ks : o.rs,
-           mn ? o.rs : o.ks, outer, inner, buf.as<uint16_t>(), ld);
-    o.p = buf.p;
-    o.mn = mn;
-    (mn ? o.ks : o.rs) = (int64_t)ld;
-    (mn ? o.rs : o.ks) = 1;
-}
+    template <class T>
+    T* at(int64_t offset) const {
+        return reinterpret_cast<T*>(buf.as<uint8_t>() + offset);
+    }
+    void place(Operand& o) const {
+        if (o.at >= 0) o.p = at<uint8_t>(o.at);
+    }
+    void allocate() {
+        if (bytes) buf.alloc(bytes);
+        if (!packs.count) return;
+        for (uint32_t c = 0; c < packs.count; ++c) packs.of[c].dst = at<uint16_t>((int64_t)pack_at[c]);
+        const uint64_t groups = packs.of[packs.count - 1].end;
+        const unsigned grid = (unsigned)std::min<uint64_t>((groups + 255) / 256, 148 * 16);
+        launch_overlapped(pack_kernel, dim3(grid), 256, 0, dim3(0), st, packs);
+    }
+    // The operand as the tensor copies can read it: as it lies (K-major, or MN-major where allowed), or a copy.
+    void settle(Operand& o, bool allow_mn) {
+        if (o.red == 1) o.ks = 1;  // a stride that no element uses
+        if (o.rows == 1) o.rs = (int64_t)round_up(o.red, 8);
+        const bool base = o.at >= 0 || aligned16(o.p);
+        if (o.ks == 1 && o.rs % 8 == 0 && o.rs >= (int64_t)o.red && base) return;
+        if (o.red == 1) o.ks = (int64_t)round_up(o.rows, 8);
+        if (allow_mn && o.rs == 1 && o.ks % 8 == 0 && o.ks >= (int64_t)o.rows && base) {
+            o.mn = true;
+            return;
+        }
+        // packed along the contiguous index, so that the copy reads and writes neighbouring elements
+        const bool mn = allow_mn && o.rs == 1 && o.ks != 1;
+        const uint64_t outer = mn ? o.red : o.rows, inner = mn ? o.rows : o.red, ld = round_up(inner, 8);
+        const uint32_t c = packs.count++;
+        packs.of[c] = {static_cast<const uint16_t*>(o.p), mn ? o.ks : o.rs, mn ? o.rs : o.ks, outer, inner, ld, nullptr,
+                       (c ? packs.of[c - 1].end : 0) + outer * (ld / 8)};
+        o.at = reserve(outer * ld * 2);
+        pack_at[c] = (uint64_t)o.at;
+        o.mn = mn;
+        (mn ? o.ks : o.rs) = (int64_t)ld;
+        (mn ? o.rs : o.ks) = 1;
+    }
+};
 
 static CUtensorMap operand_map(const Operand& o, int half, uint32_t box_rows) {
     CUtensorMap map;
@@ -1178,11 +1220,16 @@ static void launch_few(const Task& t, bool vec, cudaStream_t st) {
            static_cast<const uint16_t*>(t.q.p), t.q.rs, (uint32_t)t.p.red, t.e);
 }
 
-// The products of one call, out = epilogue(Q P^T): p the operand of the output's columns, q of its rows.
-template <bool HALF>
-static void products(Task* tasks, int count, cudaStream_t st) {
-    std::deque<DevBuf> packed;
-    uint64_t rows = 0, pair_tiles = 0;
+// Up to 4 rows with both operands contiguous along the reduction go to the streaming kernel, as they lie.
+static bool few_rows(const Task& t) { return t.e.rows <= 4 && t.p.red && t.p.ks == 1 && t.q.ks == 1; }
+// Two products share a launch, and its tiles' size, unless one has so few rows that its tiles are narrower.
+static bool together(const Task* tasks, int count) {
+    return count == 2 && std::min(tasks[0].e.rows, tasks[1].e.rows) > 64;
+}
+
+// The products of one call, out = epilogue(Q P^T), p the operand of the output's columns and q of its rows: what
+// there is to do (the number returned, moved to the front), and the scratch memory for it.
+static int plan(Task* tasks, int count, Scratch& scratch) {
     int live = 0;
     for (int i = 0; i < count; ++i) {
         Task t = tasks[i];
@@ -1197,40 +1244,51 @@ static void products(Task* tasks, int count, cudaStream_t st) {
             return fits(e.out) && fits(e.pre) && fits(e.res);
         };
         e.vec = takes(8) ? 8 : takes(4) ? 4 : 1;
-        rows = std::max(rows, e.rows);
-        pair_tiles += ((e.rows + 255) / 256) * ((e.cols + 255) / 256);
         tasks[live++] = t;
-    }
-    if (!live) return;
-    if (live == 2 && std::min(tasks[0].e.rows, tasks[1].e.rows) <= 64) {  // too unlike for tiles of one size
-        products<HALF>(tasks, 1, st);
-        products<HALF>(tasks + 1, 1, st);
-        return;
-    }
-    if (live == 1 && rows <= 4 && tasks[0].p.red && tasks[0].p.ks == 1 && tasks[0].q.ks == 1) {
-        const Task& t = tasks[0];
-        const bool vec = aligned16(t.p.p) && aligned16(t.q.p) && t.p.rs % 8 == 0 && (rows == 1 || t.q.rs % 8 == 0) &&
-                         t.p.red % 8 == 0;
-        const auto run = rows == 1 ? launch_few<HALF, 1> : rows == 2 ? launch_few<HALF, 2> : rows == 3 ? launch_few<HALF, 3> : launch_few<HALF, 4>;
-        return run(t, vec, st);
     }
     for (int i = 0; i < live; ++i) {
         Task& t = tasks[i];
+        if (few_rows(t)) continue;
         if (t.p.red) {
-            packed.emplace_back(st);
-            settle(t.p, true, packed.back(), st);
-            packed.emplace_back(st);
-            settle(t.q, rows > 32, packed.back(), st);
+            scratch.settle(t.p, true);
+            scratch.settle(t.q, t.e.rows > 32);  // (narrower boxes have no MN-major form)
         } else {  // nothing is read: any valid address and stride for the tensor maps
-            t.p.p = t.q.p = packed.emplace_back(st, 256).p;
+            t.p.at = t.q.at = scratch.reserve(256);
             t.p.rs = t.q.rs = 8;
             t.p.ks = t.q.ks = 1;
             t.p.rows = t.q.rows = 1;
         }
     }
-    const bool empty = tasks[0].p.red == 0 || tasks[live - 1].p.red == 0;
+    return live;
+}
+
+template <bool HALF>
+static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st) {
+    if (!count) return;
+    if (count == 2 && !together(tasks, count)) {
+        run<HALF>(tasks, 1, scratch, st);
+        run<HALF>(tasks + 1, 1, scratch, st);
+        return;
+    }
+    uint64_t rows = 0, pair_tiles = 0;
+    bool empty = false;
+    for (int i = 0; i < count; ++i) {
+        scratch.place(tasks[i].p);
+        scratch.place(tasks[i].q);
+        const Epilogue& e = tasks[i].e;
+        rows = std::max(rows, e.rows);
+        pair_tiles += ((e.rows + 255) / 256) * ((e.cols + 255) / 256);
+        empty = empty || tasks[i].p.red == 0;
+    }
+    if (count == 1 && few_rows(tasks[0])) {
+        const Task& t = tasks[0];
+        const bool vec = aligned16(t.p.p) && aligned16(t.q.p) && t.p.rs % 8 == 0 && (rows == 1 || t.q.rs % 8 == 0) &&
+                         t.p.red % 8 == 0;
+        const auto go = rows == 1 ? launch_few<HALF, 1> : rows == 2 ? launch_few<HALF, 2> : rows == 3 ? launch_few<HALF, 3> : launch_few<HALF, 4>;
+        return go(t, vec, st);
+    }
     if (!empty && rows > 128 && pair_tiles >= 37)
-        live == 2 ? launch_pairs<HALF, 2, 256>(tasks, st) : launch_pairs<HALF, 1, 256>(tasks, st);
+        count == 2 ? launch_pairs<HALF, 2, 256>(tasks, st) : launch_pairs<HALF, 1, 256>(tasks, st);
     else if (rows <= 16)
         launch_tiles<HALF, 1, 16, 6, 2>(tasks, st);
     else if (rows <= 32)
@@ -1238,7 +1296,7 @@ static void products(Task* tasks, int count, cudaStream_t st) {
     else if (rows <= 64)
         launch_tiles<HALF, 1, 64, 4, 2>(tasks, st);
     else
-        live == 2 ? launch_tiles<HALF, 2, 128, 3, 2>(tasks, st) : launch_tiles<HALF, 1, 128, 3, 2>(tasks, st);
+        count == 2 ? launch_tiles<HALF, 2, 128, 3, 2>(tasks, st) : launch_tiles<HALF, 1, 128, 3, 2>(tasks, st);
 }
 
 template <bool HALF>
@@ -1297,7 +1355,10 @@ static void forward(int device, const oztt_linear& a, cudaStream_t st) {
     e.bias_stride = a.bias.col_stride;
     e.act = a.activation;
     Task t{{a.w.data, a.n, a.k, a.w.row_stride, a.w.col_stride}, {a.x.data, a.m, a.k, a.x.row_stride, a.x.col_stride}, e};
-    products<HALF>(&t, 1, st);
+    Scratch scratch(st);
+    const int count = plan(&t, 1, scratch);
+    scratch.allocate();
+    run<HALF>(&t, count, scratch, st);
 }
 
 template <bool HALF>
@@ -1313,37 +1374,25 @@ static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
     check_view(a.db, false, "linear_backward: db");
     DeviceScope scope(device);
     check_earlier_calls();
-    View dz = view(a.dy);
-    DevBuf dz_buf(st), sums(st);
-    const bool has_products = (a.dx.data && a.m && a.k) || (a.dw.data && a.n && a.k);
-    if (mn && ((act && has_products) || a.db.data)) {
-        // clusters of up to 8 blocks, one below the other, as many as spread over the device; at least 16 rows a block
-        const uint64_t ld = round_up(a.n, 8), strips = (a.n + DZ_COLS - 1) / DZ_COLS, most = (a.m + DZ_ROWS - 1) / DZ_ROWS;
-        uint32_t cluster = 1;
-        while (cluster < DZ_CLUSTER && cluster * 2 <= most) cluster *= 2;
-        // (up to 128 rows a block need no second cluster, nor the launch that joins the clusters' sums)
-        const uint64_t clusters =
-            most <= 8 * cluster ? 1 : std::max<uint64_t>(1, std::min(most / cluster, (148 * 4) / (strips * cluster)));
-        const uint64_t span = round_up((a.m + clusters * cluster - 1) / (clusters * cluster), DZ_ROWS);
-        const bool store = act && has_products;
-        if (store) dz_buf.alloc(a.m * ld * 2);
-        if (a.db.data && clusters > 1) sums.alloc(clusters * a.n * 4);
-        const auto fits = [](const View& v) { return !v.p || (v.cs == 1 && v.rs % 8 == 0 && aligned16(v.p)); };
-        auto* db = static_cast<uint16_t*>(a.db.data);
-        const View z = act ? view(a.pre) : View{};
-        if (strips >= (1ull << 31)) throw Error(OZTT_EINVAL, "linear_backward: problem too large");
-        launch_overlapped(dz_variant<HALF>(fits(dz) && fits(z) && a.n % 8 == 0, a.activation),
-               dim3((unsigned)strips, (unsigned)(clusters * cluster)), 256, 0, dim3(1, cluster, 1), st, dz, z, a.m, a.n,
-               span, store ? dz_buf.as<uint16_t>() : nullptr, ld, clusters > 1 ? sums.as<float>() : nullptr,
-               clusters > 1 ? nullptr : db, a.db.col_stride);
-        if (a.db.data && clusters > 1)
-            launch_overlapped(db_kernel<HALF>, dim3((unsigned)((a.n + 31) / 32)), 256, 0, dim3(0), st, sums.as<float>(), clusters, a.n, db,
-                   a.db.col_stride);
-        if (store) dz = {dz_buf.p, (int64_t)ld, 1};
-    } else if (a.db.data && a.n) {  // no rows: zeros
-        launch_overlapped(db_kernel<HALF>, dim3((unsigned)((a.n + 31) / 32)), 256, 0, dim3(0), st, static_cast<const float*>(nullptr),
-               uint64_t{0}, a.n, static_cast<uint16_t*>(a.db.data), a.db.col_stride);
-    }
+    const View dy = view(a.dy), z = act ? view(a.pre) : View{};
+    const auto fits = [](const View& v) { return !v.p || (v.cs == 1 && v.rs % 8 == 0 && aligned16(v.p)); };
+    const bool products = mn && ((a.dx.data && a.k) || (a.dw.data && a.k));
+    // dz is written where an activation makes it, or where the products cannot read dy as it lies: one pass for both
+    // of them and for db
+    const bool write = products && (act || !fits(dy)), sum = mn && a.db.data;
+    // clusters of up to 8 blocks, one below the other, as many as spread over the device; at least 16 rows a block,
+    // and up to 128 rows a block no second cluster, nor the launch that joins the clusters' sums
+    const uint64_t ld = round_up(a.n, 8), strips = (a.n + DZ_COLS - 1) / DZ_COLS, most = (a.m + DZ_ROWS - 1) / DZ_ROWS;
+    uint32_t cluster = 1;
+    while (cluster < DZ_CLUSTER && cluster * 2 <= most) cluster *= 2;
+    uint64_t clusters = 1;
+    if (mn && most > 8 * cluster) clusters = std::max<uint64_t>(1, std::min(most / cluster, (148 * 4) / (strips * cluster)));
+    if (strips >= (1ull << 31)) throw Error(OZTT_EINVAL, "linear_backward: problem too large");
+
+    Scratch scratch(st);
+    const int64_t dz_at = write ? scratch.reserve(a.m * ld * 2) : -1;
+    const int64_t sums_at = sum && clusters > 1 ? scratch.reserve(clusters * a.n * 4) : -1;
+    const View dz = write ? View{nullptr, (int64_t)ld, 1} : dy;
     Task tasks[2];
     int count = 0;
     Epilogue e{};
@@ -1352,15 +1401,27 @@ static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
         e.rows = a.m;
         e.cols = a.k;
         e.out = view(a.dx);
-        tasks[count++] = {{a.w.data, a.k, a.n, a.w.col_stride, a.w.row_stride}, {dz.p, a.m, a.n, dz.rs, dz.cs}, e};
+        tasks[count++] = {{a.w.data, a.k, a.n, a.w.col_stride, a.w.row_stride}, {dz.p, a.m, a.n, dz.rs, dz.cs, false, dz_at}, e};
     }
     if (a.dw.data) {  // dw[n][t] = sum_i dz[i][n] x[i][t]
         e.rows = a.n;
         e.cols = a.k;
         e.out = view(a.dw);
-        tasks[count++] = {{a.x.data, a.k, a.m, a.x.col_stride, a.x.row_stride}, {dz.p, a.n, a.m, dz.cs, dz.rs}, e};
+        tasks[count++] = {{a.x.data, a.k, a.m, a.x.col_stride, a.x.row_stride}, {dz.p, a.n, a.m, dz.cs, dz.rs, false, dz_at}, e};
     }
-    products<HALF>(tasks, count, st);
+    count = plan(tasks, count, scratch);
+    scratch.allocate();
+    auto* db = static_cast<uint16_t*>(a.db.data);
+    if (write || sum)
+        launch_overlapped(dz_variant<HALF>(fits(dy) && fits(z) && a.n % 8 == 0, a.activation),
+                          dim3((unsigned)strips, (unsigned)(clusters * cluster)), 256, 0, dim3(1, cluster, 1), st, dy, z, a.m,
+                          a.n, round_up((a.m + clusters * cluster - 1) / (clusters * cluster), DZ_ROWS),
+                          write ? scratch.at<uint16_t>(dz_at) : nullptr, ld, sums_at >= 0 ? scratch.at<float>(sums_at) : nullptr,
+                          sum && sums_at < 0 ? db : nullptr, a.db.col_stride);
+    if (db && a.n && (sums_at >= 0 || !a.m))  // without rows: zeros
+        launch_overlapped(db_kernel<HALF>, dim3((unsigned)((a.n + 31) / 32)), 256, 0, dim3(0), st,
+                          a.m ? scratch.at<float>(sums_at) : nullptr, a.m ? clusters : 0, a.n, db, a.db.col_stride);
+    run<HALF>(tasks, count, scratch, st);
 }
 
 }  // namespace layer
