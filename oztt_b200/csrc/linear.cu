@@ -314,40 +314,47 @@ __device__ __forceinline__ void finish_vector(uint16_t* out, uint16_t* pre, bool
     for (int q = 0; q < N; ++q) w[q] = pack<HALF>(z[q]);
     store_words(out, w);
 }
-// The same for any N values, (di, dj) apart, of which those inside the output are finished, by accesses of one value.
-template <bool HALF, int N>
-__device__ __forceinline__ void finish_scattered(const Epilogue& e, uint64_t i, uint64_t j, uint32_t di, uint32_t dj,
-                                                 const float (&sums)[N]) {
-    uint16_t r[N + 1];
-    bool in[N + 1];
-    f32x2 z[(N + 1) / 2];
-#pragma unroll
-    for (int q = 0; q < N; ++q) {
-        in[q] = i + q * di < e.rows && j + q * dj < e.cols;
-        r[q] = e.res.p && in[q] ? *element(e.res, i + q * di, j + q * dj) : 0;
+// A lane's values by accesses of one value: where the first of them lies in each view, and how far apart they are.
+struct Scattered {
+    uint16_t *out, *pre;
+    const uint16_t* res;
+    int64_t out_step, pre_step, res_step;
+    // from (i, j) on, in steps of di rows and dj columns
+    __device__ __forceinline__ Scattered(const Epilogue& e, uint64_t i, uint64_t j, int64_t di, int64_t dj)
+        : out(element(e.out, i, j)), pre(e.pre.p ? element(e.pre, i, j) : nullptr), res(e.res.p ? element(e.res, i, j) : nullptr),
+          out_step(di * e.out.rs + dj * e.out.cs), pre_step(di * e.pre.rs + dj * e.pre.cs),
+          res_step(di * e.res.rs + dj * e.res.cs) {}
+    template <int N>
+    __device__ __forceinline__ void advance() {
+        out += N * out_step;
+        if (pre) pre += N * pre_step;
+        if (res) res += N * res_step;
     }
-    in[N] = false;
+};
+// The same as finish_vector for N values, of which the first `count` are inside the output.
+template <bool HALF, int N>
+__device__ __forceinline__ void finish_scattered(const Scattered& at, uint32_t count, int act, const float (&sums)[N]) {
+    uint16_t r[N];
+    f32x2 z[(N + 1) / 2];
+    const auto each = [&](auto* p, int64_t step, auto&& f) {
+#pragma unroll
+        for (uint32_t q = 0; q < N; ++q, p += step)
+            if (q < count) f(p, q);
+    };
+    if (at.res) each(at.res, at.res_step, [&](const uint16_t* p, uint32_t q) { r[q] = *p; });
 #pragma unroll
     for (int q = 0; q < (N + 1) / 2; ++q) z[q] = pk2(sums[2 * q], 2 * q + 1 < N ? sums[2 * q + 1 < N ? 2 * q + 1 : 0] : 0.0f);
-    const auto store = [&](const View& v) {
-#pragma unroll
-        for (int q = 0; q < N; ++q) {
-            const uint32_t w = pack<HALF>(z[q / 2]);
-            if (in[q]) *element(v, i + q * di, j + q * dj) = (uint16_t)(w >> (16 * (q & 1)));
-        }
+    const auto store = [&](uint16_t* p, int64_t step) {
+        each(p, step, [&](uint16_t* to, uint32_t q) { *to = (uint16_t)(pack<HALF>(z[q / 2]) >> (16 * (q & 1))); });
     };
-    if (e.pre.p) store(e.pre);
-    activate_all(z, e.act);
-    if (e.res.p) {
+    if (at.pre) store(at.pre, at.pre_step);
+    activate_all(z, act);
+    if (at.res) {
 #pragma unroll
-        for (int q = 0; q < N; ++q) {
-            float lo, hi;
-            unpk2(z[q / 2], lo, hi);
-            const float y = ((q & 1) ? hi : lo) + to_f32<HALF>(r[q]);
-            z[q / 2] = (q & 1) ? pk2(lo, y) : pk2(y, hi);
-        }
+        for (int q = 0; q < (N + 1) / 2; ++q)
+            z[q] = add2(z[q], pk2(to_f32<HALF>(r[2 * q]), 2 * q + 1 < N ? to_f32<HALF>(r[2 * q + 1 < N ? 2 * q + 1 : 0]) : 0.0f));
     }
-    store(e.out);
+    store(at.out, at.out_step);
 }
 template <bool HALF>
 __device__ __forceinline__ float bias_at(const Epilogue& e, uint64_t j) {
@@ -515,7 +522,9 @@ __global__ void __launch_bounds__(THREADS, CTAS)
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) z[q] += acc[q];
-            finish_scattered<HALF, 4>(e, i, col[0], 0, 32, z);
+            if (col[0] < e.cols)
+                finish_scattered<HALF, 4>(Scattered(e, i, col[0], 0, 32), (uint32_t)min((e.cols - col[0] + 31) / 32, (uint64_t)4),
+                                          e.act, z);
         }
     }
     __syncthreads();
@@ -768,6 +777,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     res += PATCH_ROWS * e.res.rs;
                 }
             } else {
+                Scattered at(e, i0, j0 + lane, 1, 0);
 #pragma unroll 1
                 for (uint32_t c = 0; c < rows; c += PATCH_ROWS) {
                     uint32_t v[8];
@@ -775,7 +785,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     float z[8];
 #pragma unroll
                     for (int q = 0; q < 8; ++q) z[q] = __uint_as_float(v[q]) + lane_bias;
-                    finish_scattered<HALF, 8>(e, i0 + c, j0 + lane, 1, 0, z);
+                    finish_scattered<HALF, 8>(at, j0 + lane < e.cols ? rows - c : 0, e.act, z);
+                    at.advance<8>();
                 }
             }
             // the sums have been read: all that the arrival has to tell; a releasing one would also
@@ -879,7 +890,7 @@ __global__ void __launch_bounds__(256)
         const uint64_t i = threadIdx.x / FEW_COLS, j = j0 + threadIdx.x % FEW_COLS;
         float z[1] = {bias_at<HALF>(e, j)};
         for (uint32_t w = 0; w < warps; ++w) z[0] += sums[w][threadIdx.x];
-        finish_scattered<HALF, 1>(e, i, j, 0, 0, z);
+        if (j < e.cols) finish_scattered<HALF, 1>(Scattered(e, i, j, 0, 0), 1, e.act, z);
     }
 }
 
@@ -1270,7 +1281,7 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
         run<HALF>(tasks + 1, 1, scratch, st);
         return;
     }
-    uint64_t rows = 0, pair_tiles = 0;
+    uint64_t rows = 0, pair_tiles = 0, tiles = 0, blocks = 0;
     bool empty = false;
     for (int i = 0; i < count; ++i) {
         scratch.place(tasks[i].p);
@@ -1278,6 +1289,8 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
         const Epilogue& e = tasks[i].e;
         rows = std::max(rows, e.rows);
         pair_tiles += ((e.rows + 255) / 256) * ((e.cols + 255) / 256);
+        tiles += ((e.rows + 127) / 128) * ((e.cols + 127) / 128);
+        blocks = std::max(blocks, (tasks[i].p.red + BK - 1) / BK);
         empty = empty || tasks[i].p.red == 0;
     }
     if (count == 1 && few_rows(tasks[0])) {
@@ -1287,14 +1300,22 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
         const auto go = rows == 1 ? launch_few<HALF, 1> : rows == 2 ? launch_few<HALF, 2> : rows == 3 ? launch_few<HALF, 3> : launch_few<HALF, 4>;
         return go(t, vec, st);
     }
-    if (!empty && rows > 128 && pair_tiles >= 37)
+    // Which tiles, by what was measured (us, BF16, single products):
+    //   output      sum    64 rows  128 rows  pairs
+    //   512x4096    1024     12.1     13.3     11.5      pairs from half the device's SMs on, and from a third where
+    //   512x4096    4096     26.8     23.7     27.3      the sum is short (up to 24 blocks): their tiles need a third
+    //   1024x4096   4096     52.3     37.7     28.9      of the bytes from L2, but leave more SMs idle when few
+    //   512x2048    1024      9.8     10.5     11.2      64 rows where 128 would leave most SMs idle or the sum is
+    //   256x2048    4096     12.0     13.7     25.6      short, since the CTAs of a split sum join sooner
+    //   512x2048    4096     17.2     15.9     26.1
+    if (!empty && rows > 128 && (pair_tiles >= 37 || (pair_tiles >= 24 && blocks <= 24)))
         count == 2 ? launch_pairs<HALF, 2, 256>(tasks, st) : launch_pairs<HALF, 1, 256>(tasks, st);
     else if (rows <= 16)
         launch_tiles<HALF, 1, 16, 6, 2>(tasks, st);
     else if (rows <= 32)
         launch_tiles<HALF, 1, 32, 5, 2>(tasks, st);
-    else if (rows <= 64)
-        launch_tiles<HALF, 1, 64, 4, 2>(tasks, st);
+    else if (rows <= 64 || tiles <= 32 || blocks <= 24)
+        count == 2 ? launch_tiles<HALF, 2, 64, 4, 2>(tasks, st) : launch_tiles<HALF, 1, 64, 4, 2>(tasks, st);
     else
         count == 2 ? launch_tiles<HALF, 2, 128, 3, 2>(tasks, st) : launch_tiles<HALF, 1, 128, 3, 2>(tasks, st);
 }
