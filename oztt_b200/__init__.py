@@ -214,6 +214,7 @@ _SIGNATURES = {
     "oztt_get_option": [_I32, ctypes.POINTER(_I32)],
     "oztt_is_available": [_I32],
     "oztt_format_name": [_I32],
+    "oztt_test_linear_error": [_I32, _ERR, _SZ],
     "oztt_test_udiv_small": [ctypes.c_uint32, ctypes.c_uint32],
     "oztt_test_ext80_dot": [_P, _P, _U64, ctypes.c_double],
     "oztt_test_gemm_wait_timeout": [_U64, _P, _P, _ERR, _SZ],

@@ -118,6 +118,22 @@ def test_forward_large_layouts(oztt, cuda, layout):
     check_forward(oztt, x, w, b, r.t().contiguous().t(), "silu", pre=True)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,k", [(300, 77), (1, 4097), (5, 16390), (2049, 515)])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5])
+def test_forward_few_rows_unaligned(oztt, cuda, dtype, m, n, k):
+    x, w, b, r = make(m, n, k, dtype, seed=m)
+    check_forward(oztt, x, w, b, r, "silu", pre=True)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 9])
+def test_backward_few_rows(oztt, cuda, m):
+    x, w, b, dy = make(m, 520, 264, torch.bfloat16, seed=m)
+    check_backward(oztt, dy, x, w, dy.roll(1, 1), "gelu")
+    x, w, b, dy = make(m, 515, 77, torch.float16, seed=m)
+    check_backward(oztt, dy, x, w, None, "none")
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_forward_activations(oztt, cuda, act, dtype):
@@ -327,6 +343,15 @@ def test_gradient_against_differences(oztt, cuda, act):
         rounding = U[dt] * float((g.double() * step).abs().sum())
         curve = 2 * float((dy.double().abs() * zdot.abs() ** 3).sum())
         assert abs(float(val[0] - val[1]) / 2 - want) <= 4 * spread + rounding + curve, name
+
+
+def test_a_wait_that_gave_up_is_reported_once(oztt, cuda):
+    x, w, b, r = make(8, 96, 80, torch.bfloat16)
+    want = oztt.linear(x, w, b)
+    oztt.call("oztt_test_linear_error", 2)
+    with pytest.raises(RuntimeError, match="earlier call gave up waiting"):
+        oztt.linear(x, w, b)
+    assert torch.equal(oztt.linear(x, w, b), want)
 
 
 def test_refusals(oztt, cuda):

@@ -22,6 +22,7 @@ def backward(oztt, fmt=0, act=0, m=4, n=4, k=8, dy=SOME, pre=NONE, x=SOME, w=SOM
                                      (dict(x=NONE), "x is missing"), (dict(w=NONE), "w is missing"),
                                      (dict(y=NONE), "y is missing"), (dict(x=(4097, 8, 1)), "aligned"),
                                      (dict(w=(4096, -8, 1)), "negative"), (dict(b=(4096, 0, -1)), "negative"),
+                                     (dict(y=(4096, 0, 1)), "must not be zero"), (dict(pre=(4096, 8, 0)), "must not be zero"),
                                      (dict(device=-1), "device_id")])
 def test_forward_refusals(oztt, kw, text):
     with pytest.raises(ValueError, match=text):
@@ -31,7 +32,8 @@ def test_forward_refusals(oztt, kw, text):
 @pytest.mark.parametrize("kw,text", [(dict(fmt=4), "BF16 or FP16"), (dict(act=9), "activation"),
                                      (dict(act=2), "pre"), (dict(dy=NONE), "dy is missing"),
                                      (dict(x=NONE), "x is missing"), (dict(w=NONE), "w is missing"),
-                                     (dict(dx=(4099, 8, 1)), "aligned"), (dict(device=-3), "device_id")])
+                                     (dict(dx=(4099, 8, 1)), "aligned"), (dict(dw=(4096, 0, 1)), "must not be zero"),
+                                     (dict(db=(4096, 0, 0)), "must not be zero"), (dict(device=-3), "device_id")])
 def test_backward_refusals(oztt, kw, text):
     with pytest.raises(ValueError, match=text):
         backward(oztt, **kw)
