@@ -58,13 +58,14 @@ inline void launch_overlapped(void (*kernel)(Params...), dim3 grid, uint32_t thr
     OZTT_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
 }
 
-// Allows a kernel its dynamic shared memory, once on each device.
+// Allows a kernel its dynamic shared memory, and clusters of up to 16, once on each device.
 template <class Kernel>
-inline void allow_smem(Kernel* kernel, uint32_t bytes, std::atomic<uint64_t>& allowed) {
+inline void allow_smem(Kernel* kernel, uint32_t bytes, std::atomic<uint64_t>& allowed, bool large_clusters = false) {
     int device = 0;
     OZTT_CUDA(cudaGetDevice(&device));
     if (device < 64 && (allowed.load() >> device & 1)) return;
     OZTT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (large_clusters) OZTT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     if (device < 64) allowed.fetch_or(1ull << device);
 }
 

@@ -38,7 +38,7 @@ constexpr uint32_t P_BYTES = BP * BK * 2;
 constexpr uint32_t THREADS = 192;       // warp 0 loads, warp 1 issues the products, warps 2-5 read the sums
 constexpr uint32_t MN_BOX = 64;         // rows of one MN-major box: 128 bytes
 constexpr uint32_t MN_BOX_BYTES = MN_BOX * BK * 2;
-constexpr uint32_t MAX_SPLIT = 8;       // CTAs of a cluster that share one tile's reduction
+constexpr uint32_t MAX_SPLIT = 16;      // CTAs of a cluster that share one tile's reduction
 
 // A 16-bit matrix by its pointer and strides in elements.
 struct View {
@@ -1202,13 +1202,14 @@ static void launch_tiles(const Task* tasks, cudaStream_t st) {
     constexpr uint32_t SMEM = STAGES * (P_BYTES + BQ * BK * 2) + 256 + 1024;
     static std::atomic<uint64_t> allowed{0};
     auto* kernel = product_kernel<HALF, COUNT, BQ, STAGES, CTAS>;
-    allow_smem(kernel, SMEM, allowed);
+    allow_smem(kernel, SMEM, allowed, true);
     const Products<COUNT> ps = describe_all<HALF, COUNT>(tasks, BP, BQ, BQ);
-    // With few tiles the reduction is shared by up to 8 CTAs, as long as the CTAs are resident at once and each
-    // keeps at least four blocks of it.
+    // With few tiles the reduction is shared by up to 8 CTAs, as long as the CTAs are resident at once and each keeps at
+    // least two blocks of it; by 16 where that takes one CTA an SM at most, since few clusters of 16 find room in the
+    // device's parts at once (16 x 512 x 16384: 12.4 us with 8, 8.7 with 16; 128 x 1024 x 4096: 8.7 and 13.9).
     const uint32_t shortest = std::min(ps.of[0].num_kb, ps.of[COUNT - 1].num_kb);
     uint32_t split = 1;
-    while (split < MAX_SPLIT && ps.tiles * split * 2 <= 148 * CTAS && shortest / (split * 2) >= 4) split *= 2;
+    while (split < MAX_SPLIT && ps.tiles * split * 2 <= (split < 8 ? 148 * CTAS : 148) && shortest / (split * 2) >= 2) split *= 2;
     launch_overlapped(kernel, dim3(ps.tiles * split), THREADS, SMEM, dim3(split), st, ps, error_word());
 }
 
