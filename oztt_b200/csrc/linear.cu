@@ -1243,9 +1243,17 @@ static bool takes_vectors(const Task& t) {
 static bool few_rows(const Task& t) {
     return t.p.red && t.p.ks == 1 && t.q.ks == 1 && (t.e.rows == 1 || (t.e.rows <= 4 && !takes_vectors(t)));
 }
-// Two products share a launch, and its tiles' size, unless one has so few rows that its tiles are narrower.
+static uint64_t blocks_of(const Task& t) { return (t.p.red + BK - 1) / BK; }
+static uint64_t pair_tiles_of(const Task& t) { return ((t.e.rows + 255) / 256) * ((t.e.cols + 255) / 256); }
+// Two products share a launch, and its tiles' size, where one launch less counts or their tiles fill up one another's
+// waves: with short sums, or few tiles that still keep every pair busy as long as the longest sum lasts. (dx + dw, us,
+// one launch and two: 512 x 1024 x 1024 11 and 16, 1024^3 12.7 and 19.0, 2048^3 30.6 and 33.9, but 8192 x 1024 x 1024 58
+// and 41, 8192 x 16384 x 4096 1922 and 1706: pairs that work on products of unlike length drift apart, and what one has
+// read has left L2 when the next wants it.) One with few rows takes narrower tiles.
 static bool together(const Task* tasks, int count) {
-    return count == 2 && std::min(tasks[0].e.rows, tasks[1].e.rows) > 64;
+    if (count < 2 || std::min(tasks[0].e.rows, tasks[1].e.rows) <= 64) return false;
+    const uint64_t b0 = blocks_of(tasks[0]), b1 = blocks_of(tasks[1]), t0 = pair_tiles_of(tasks[0]), t1 = pair_tiles_of(tasks[1]);
+    return std::max(b0, b1) <= 24 || (t0 + t1 <= 148 && t0 * b0 + t1 * b1 >= 52 * std::max(b0, b1));
 }
 
 // The products of one call, out = epilogue(Q P^T), p the operand of the output's columns and q of its rows: what
@@ -1291,6 +1299,7 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
         run<HALF>(tasks + 1, 1, scratch, st);
         return;
     }
+    if (count == 2 && tasks[1].p.red > tasks[0].p.red) std::swap(tasks[0], tasks[1]);  // the longest tiles first
     uint64_t rows = 0, pair_tiles = 0, tiles = 0, blocks = 0;
     bool empty = false;
     for (int i = 0; i < count; ++i) {
@@ -1298,9 +1307,9 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
         scratch.place(tasks[i].q);
         const Epilogue& e = tasks[i].e;
         rows = std::max(rows, e.rows);
-        pair_tiles += ((e.rows + 255) / 256) * ((e.cols + 255) / 256);
+        pair_tiles += pair_tiles_of(tasks[i]);
         tiles += ((e.rows + 127) / 128) * ((e.cols + 127) / 128);
-        blocks = std::max(blocks, (tasks[i].p.red + BK - 1) / BK);
+        blocks = std::max(blocks, blocks_of(tasks[i]));
         empty = empty || tasks[i].p.red == 0;
     }
     if (count == 1 && few_rows(tasks[0])) {
