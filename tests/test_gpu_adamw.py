@@ -82,6 +82,33 @@ def test_steps_of_32_bits(oztt, cuda, param, grad, master, offset):
                 within(params[i], p2, U[param] * p2.abs() + (1 + U[param]) * dp + TINY[param], "p")
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("offset", range(1, 9))
+def test_every_alignment(oztt, cuda, bits, offset):
+    """Parameters and gradients at every address give what aligned ones give, bit for bit, and nothing beside them is
+    written."""
+    sizes = [1, 255, 256, 300, 4096, 9001]
+    runs = []
+    for off in (0, offset):
+        for dtype in (torch.bfloat16, torch.float32):
+            params, grads = [], []
+            for n, v, g in zip(sizes, tensors(sizes, dtype, 1), tensors(sizes, dtype, 2)):
+                room = torch.full((n + 32,), 7.0, dtype=dtype, device="cuda")
+                params.append(room[8 + off:8 + off + n].copy_(v))
+                grads.append(torch.full((n + 32,), 7.0, dtype=dtype, device="cuda")[24 - off:24 - off + n].copy_(g))
+            opt = oztt.AdamW(params, state_bits=bits, seed=3, **HYPER)
+            for _ in range(2):
+                opt.step(grads)
+            for p, n in zip(params, sizes):
+                whole = p._base
+                beside = torch.cat([whole[:8 + off], whole[8 + off + n:]])
+                assert bool((beside == 7.0).all())
+            runs.append((params, *opt.moments()))
+    for aligned, other in ((runs[0], runs[2]), (runs[1], runs[3])):
+        assert all(torch.equal(a, b) for a, b in zip(aligned[0], other[0]))
+        assert torch.equal(aligned[1], other[1]) and torch.equal(aligned[2], other[2])
+
+
 def random_bits(n, seed):
     mask = np.uint64(0xFFFFFFFF)
     h = (np.arange(n, dtype=np.uint64) * np.uint64(0x9E3779B9) + np.uint64(seed & 0xFFFFFFFF)) & mask
