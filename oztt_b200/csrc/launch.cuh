@@ -19,10 +19,14 @@ struct DeviceScope {
             changed = true;
         }
         static std::atomic<uint64_t> opened{0};
-        if (device < 64 && !(opened.load() >> device & 1)) {
+        if (device < 64 && (opened.load() >> device & 1)) return;
+        try {
             open_device(device);
-            opened.fetch_or(1ull << device);
+        } catch (...) {
+            cudaSetDevice(before);
+            throw;
         }
+        if (device < 64) opened.fetch_or(1ull << device);
     }
     ~DeviceScope() {
         if (changed) cudaSetDevice(before);

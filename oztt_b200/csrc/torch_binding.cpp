@@ -235,40 +235,55 @@ int32_t type_of(const at::Tensor& t) {
     }
 }
 
-// adamw_step(table, grads, grad_scale, moments, hyper, device): table a writable buffer of oztt_adamw_tensor, one for
-// each parameter, whose gradients are filled in here; grads a list or tuple; moments and hyper bytes of
-// oztt_adamw_moments and oztt_adamw_hyper (with grad_scale filled in here).
+// The items of a list or tuple of n.
+PyObject** items(PyObject* o, Py_ssize_t n, const char* what) {
+    if (!PyList_Check(o) && !PyTuple_Check(o)) refuse(std::string("AdamW: ") + what + " must be a list or a tuple");
+    if (PySequence_Fast_GET_SIZE(o) != n) refuse(std::string("AdamW: ") + what + " must be as many as params");
+    return PySequence_Fast_ITEMS(o);
+}
+
+// adamw_step(table, params, masters, grads, grad_scale, moments, hyper, device): table a writable buffer of
+// oztt_adamw_tensor, one for each parameter, with the count and type that it was made for; the addresses, which a
+// program may change between steps, are filled in here. masters and grads may hold None; moments and hyper are bytes
+// of oztt_adamw_moments and oztt_adamw_hyper (with grad_scale filled in here).
 PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
-    if (!expect(count, 6, "adamw_step")) return nullptr;
+    if (!expect(count, 8, "adamw_step")) return nullptr;
     Py_buffer table;
     if (PyObject_GetBuffer(args[0], &table, PyBUF_WRITABLE) != 0) return nullptr;
     PyObject* result = guarded([&]() -> PyObject* {
         auto* t = static_cast<oztt_adamw_tensor*>(table.buf);
         const Py_ssize_t n = table.len / (Py_ssize_t)sizeof(oztt_adamw_tensor);
-        if (!PyList_Check(args[1]) && !PyTuple_Check(args[1])) refuse("AdamW: grads must be a list or a tuple");
-        if (PySequence_Fast_GET_SIZE(args[1]) != n) refuse("AdamW: grads must be as many as params");
-        PyObject** grads = PySequence_Fast_ITEMS(args[1]);
-        const int device = (int)PyLong_AsLong(args[5]);
+        PyObject **params = items(args[1], n, "params"), **masters = items(args[2], n, "masters"),
+                 **grads = items(args[3], n, "grads");
+        const int device = (int)PyLong_AsLong(args[7]);
         for (Py_ssize_t i = 0; i < n; ++i) {
-            const at::Tensor* g = tensor_or_none(grads[i], "AdamW", "a gradient");
+            const auto address = [&](const at::Tensor& x, const char* what) -> void* {
+                const auto which = [&] { return std::string("AdamW: ") + what + " " + std::to_string(i); };
+                if (!x.is_cuda() || x.get_device() != device) refuse(which() + " must be on the parameters' device");
+                if ((uint64_t)x.numel() != t[i].count) refuse(which() + " has not its parameter's size");
+                if (!x.is_contiguous()) refuse(which() + " must be contiguous");
+                return x.data_ptr();
+            };
             t[i].grad = nullptr;
+            const at::Tensor* g = tensor_or_none(grads[i], "AdamW", "a gradient");
             if (!g) continue;
-            const int32_t type = type_of(*g);
-            const auto which = [&] { return "AdamW: gradient " + std::to_string(i); };
-            if (type < 0) refuse(which() + " must be BF16, FP16 or FP32");
-            if (!g->is_cuda() || g->get_device() != device) refuse(which() + " must be on the parameters' device");
-            if ((uint64_t)g->numel() != t[i].count) refuse(which() + "'s size is not its parameter's");
-            if (!g->is_contiguous()) refuse(which() + " must be contiguous");
-            t[i].grad = g->data_ptr();
-            t[i].grad_type = type;
+            t[i].grad_type = type_of(*g);
+            if (t[i].grad_type < 0) refuse("AdamW: gradient " + std::to_string(i) + " must be BF16, FP16 or FP32");
+            t[i].grad = address(*g, "gradient");
+            const at::Tensor& p = tensor(params[i], "AdamW", "a parameter");
+            if (type_of(p) != t[i].param_type) refuse("AdamW: parameter " + std::to_string(i) + " has changed its type");
+            t[i].param = address(p, "parameter");
+            const at::Tensor* w = tensor_or_none(masters[i], "AdamW", "a master");
+            if (w && w->scalar_type() != at::kFloat) refuse("AdamW: master " + std::to_string(i) + " must be FP32");
+            t[i].master = w ? static_cast<float*>(address(*w, "master")) : nullptr;
         }
         oztt_adamw_moments moments;
         oztt_adamw_hyper hyper;
-        if (PyBytes_GET_SIZE(args[3]) != sizeof moments || PyBytes_GET_SIZE(args[4]) != sizeof hyper)
+        if (PyBytes_GET_SIZE(args[5]) != sizeof moments || PyBytes_GET_SIZE(args[6]) != sizeof hyper)
             throw std::runtime_error("adamw_step: records of another size");
-        std::memcpy(&moments, PyBytes_AS_STRING(args[3]), sizeof moments);
-        std::memcpy(&hyper, PyBytes_AS_STRING(args[4]), sizeof hyper);
-        if (const at::Tensor* s = tensor_or_none(args[2], "AdamW", "grad_scale")) {
+        std::memcpy(&moments, PyBytes_AS_STRING(args[5]), sizeof moments);
+        std::memcpy(&hyper, PyBytes_AS_STRING(args[6]), sizeof hyper);
+        if (const at::Tensor* s = tensor_or_none(args[4], "AdamW", "grad_scale")) {
             if (s->scalar_type() != at::kFloat || !s->is_cuda() || s->get_device() != device || s->numel() != 1)
                 refuse("AdamW: grad_scale must be one FP32 number on the parameters' device");
             hyper.grad_scale = s->const_data_ptr<float>();

@@ -21,7 +21,7 @@ _TENSOR = np.dtype([("param", np.uint64), ("grad", np.uint64), ("master", np.uin
 _MOMENTS = struct.Struct("=i4x4Q")
 _HYPER = struct.Struct("=5dQQI4x")
 
-_torch = _binding()  # csrc/torch_binding.cpp: the gradients' checks and addresses, the current stream
+_torch = _binding()  # csrc/torch_binding.cpp: the tensors' checks and addresses, the current stream
 
 
 class AdamW:
@@ -77,18 +77,16 @@ class AdamW:
         self.offsets = [BLOCK * (sum_ - b) for b, sum_ in zip(blocks, np.cumsum(blocks).tolist())]
         kind = torch.uint8 if state_bits == 8 else torch.float32
         zeros = lambda n, dtype: torch.zeros(n, dtype=dtype, device=device)  # noqa: E731
-        self.m, self.v = zeros(self.blocks * BLOCK, kind), zeros(self.blocks * BLOCK, kind)
-        self.m_exp = self.v_exp = None
+        self._m, self._v = zeros(self.blocks * BLOCK, kind), zeros(self.blocks * BLOCK, kind)
+        self._m_exp = self._v_exp = None
         if state_bits == 8:
-            self.m_exp, self.v_exp = zeros(self.blocks, kind), zeros(self.blocks, kind)
+            self._m_exp, self._v_exp = zeros(self.blocks, kind), zeros(self.blocks, kind)
         self._table = np.zeros(len(params), _TENSOR)
-        self._table["param"] = [p.data_ptr() for p in params]
-        self._table["master"] = [0 if w is None else w.data_ptr() for w in masters]
         self._table["count"] = self._counts
         self._table["param_type"] = [_TYPES[p.dtype] for p in params]
         self._grown = [p for p in params if p.requires_grad]
-        exps = (self.m_exp.data_ptr(), self.v_exp.data_ptr()) if state_bits == 8 else (0, 0)
-        self._record = _MOMENTS.pack(state_bits, self.m.data_ptr(), self.v.data_ptr(), *exps)
+        exps = (self._m_exp.data_ptr(), self._v_exp.data_ptr()) if state_bits == 8 else (0, 0)
+        self._record = _MOMENTS.pack(state_bits, self._m.data_ptr(), self._v.data_ptr(), *exps)
 
     def step(self, grads=None, *, grad_scale: torch.Tensor | None = None, lr: float | None = None,
              seed: int | None = None) -> None:
@@ -105,16 +103,23 @@ class AdamW:
             seed = self.seed + 0x632BE5AB * t
         hyper = _HYPER.pack(self.lr if lr is None else lr, *self.betas, self.eps, self.weight_decay, t,
                             0, seed & 0xFFFFFFFF)
-        _torch.adamw_step(self._table, grads, grad_scale, self._record, hyper, self.device.index)
+        _torch.adamw_step(self._table, self.params, self.masters, grads, grad_scale, self._record, hyper,
+                          self.device.index)
         self.t = t
         if self._grown:  # saved for a backward pass that has not run, they are no longer what was saved
             torch.autograd.graph.increment_version(self._grown)
+
+    # The moments as they are kept: FP32, or bytes with the blocks' exponents.
+    m = property(lambda self: self._m)
+    v = property(lambda self: self._v)
+    m_exp = property(lambda self: self._m_exp)
+    v_exp = property(lambda self: self._v_exp)
 
     def moments(self) -> tuple[torch.Tensor, torch.Tensor]:
         """The flat moments (m, v), tensor i's from offsets[i] on: the FP32 buffers themselves with 32 bits, new
         BF16 tensors with 8, which hold the values of the codes exactly."""
         if self.state_bits == 32:
-            return self.m, self.v
+            return self._m, self._v
         m, v = (torch.empty(self.blocks * BLOCK, dtype=torch.bfloat16, device=self.device) for _ in range(2))
         err = _errbuf()
         rc = _lib().oztt_adamw_values(self.device.index, self._record, self.blocks, m.data_ptr(), v.data_ptr(),
@@ -126,21 +131,21 @@ class AdamW:
     def state_dict(self) -> dict:
         """What load_state_dict needs to go on from here: the number of steps, the moments as they are kept, and the
         masters. The tensors are the optimiser's own."""
-        d = {"t": self.t, "state_bits": self.state_bits, "seed": self.seed, "m": self.m, "v": self.v,
+        d = {"t": self.t, "state_bits": self.state_bits, "seed": self.seed, "m": self._m, "v": self._v,
              "masters": self.masters}
         if self.state_bits == 8:
-            d["m_exp"], d["v_exp"] = self.m_exp, self.v_exp
+            d["m_exp"], d["v_exp"] = self._m_exp, self._v_exp
         return d
 
     def load_state_dict(self, d: dict) -> None:
         """Copies a state_dict of an optimiser of like tensors and bits."""
         names = ["m", "v"] + (["m_exp", "v_exp"] if self.state_bits == 8 else [])
-        if d.get("state_bits") != self.state_bits or any(d[n].shape != getattr(self, n).shape for n in names):
+        if d.get("state_bits") != self.state_bits or any(d[n].shape != getattr(self, "_" + n).shape for n in names):
             raise ValueError("AdamW: the state is of other tensors or bits")
         if [w is None for w in d["masters"]] != [w is None for w in self.masters]:
             raise ValueError("AdamW: the state has other masters")
         for n in names:
-            getattr(self, n).copy_(d[n])
+            getattr(self, "_" + n).copy_(d[n])
         for w, s in zip(self.masters, d["masters"]):
             if w is not None:
                 w.copy_(s)

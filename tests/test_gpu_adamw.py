@@ -304,6 +304,30 @@ def test_step_uses_grad_attributes_and_other_streams(oztt, cuda):
     assert torch.equal(p.detach(), q) and p._version > version
 
 
+def test_parameters_that_moved(oztt, cuda):
+    """A parameter given other memory between steps is stepped where it lies now; one that changed its kind is
+    refused, and nothing is stepped."""
+    p = torch.ones(500, device="cuda")
+    q = p.clone()
+    g = tensors([500], torch.float32, 2)[0]
+    a, b = oztt.AdamW([p]), oztt.AdamW([q])
+    for opt in (a, b):
+        opt.step([g])
+    old = p.data
+    kept = old.clone()
+    p.data = p.data.clone()
+    for opt in (a, b):
+        opt.step([g])
+    assert torch.equal(p, q) and torch.equal(old, kept)
+    for other in (p.data.half(), p.data[:499], torch.zeros(1000, device="cuda")[::2]):
+        before = p.data
+        p.data = other
+        with pytest.raises(ValueError):
+            a.step([g])
+        p.data = before
+    assert a.t == 2 and torch.equal(p, q)
+
+
 def test_refusals(oztt, cuda):
     p = torch.zeros(64, device="cuda")
     wide = torch.zeros(64, 2, device="cuda")
