@@ -900,35 +900,73 @@ __global__ void __launch_bounds__(256)
 
 // Copies of operands whose base or rows do not start on 16 bytes, which the tensor copies cannot read:
 // dst[o][i] = src[o * so + i * si], rows ld apart (a multiple of 8, zero beyond `inner`). Up to 4 in one launch.
+// Bound by memory: a warp takes 1024 elements of a row by aligned 16-byte loads and shifts them to their places, all
+// loads ahead of the first store. 4095 x 4097 and 16 x 4097 together: 12.6 us of a call (67 MB moved, 5.3 TB/s).
 struct Pack {
     const uint16_t* src;
     int64_t so, si;
     uint64_t outer, inner, ld;
     uint16_t* dst;
-    uint64_t end;  // groups of 8 elements of this copy and those before it
+    uint64_t end;  // units of this copy and those before it: PACK_GROUPS groups of 8 elements of a row
 };
 struct Packs {
     Pack of[4];
     uint32_t count;
 };
+constexpr uint32_t PACK_AHEAD = 4, PACK_GROUPS = 32 * PACK_AHEAD;
 __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs packs) {
+    const uint32_t lane = threadIdx.x & 31;
     overlap_launches();
-    const uint64_t all = packs.of[packs.count - 1].end;
-    for (uint64_t t = blockIdx.x * (uint64_t)blockDim.x + threadIdx.x; t < all; t += (uint64_t)gridDim.x * blockDim.x) {
+    const uint64_t all = packs.of[packs.count - 1].end, step = (uint64_t)gridDim.x * (blockDim.x >> 5);
+    for (uint64_t t = blockIdx.x * (uint64_t)(blockDim.x >> 5) + (threadIdx.x >> 5); t < all; t += step) {
         uint32_t c = 0;
         while (t >= packs.of[c].end) ++c;
         const Pack& k = packs.of[c];
-        const uint64_t g = t - (c ? packs.of[c - 1].end : 0), per_row = k.ld / 8;
-        const uint64_t o = (g | per_row) >> 32 ? g / per_row : (uint32_t)g / (uint32_t)per_row, i = (g - o * per_row) * 8;
-        const uint16_t* src = k.src + (int64_t)o * k.so + (int64_t)i * k.si;
-        uint32_t w[4];
+        const uint64_t unit = t - (c ? packs.of[c - 1].end : 0), per_row = (k.ld / 8 + PACK_GROUPS - 1) / PACK_GROUPS;
+        const uint64_t o = (unit | per_row) >> 32 ? unit / per_row : (uint32_t)unit / (uint32_t)per_row;
+        const uint64_t i0 = ((unit - o * per_row) * PACK_GROUPS + lane) * 8;
+        const uint16_t* row = k.src + (int64_t)o * k.so;
+        uint16_t* to = k.dst + o * k.ld;
+        uint32_t v[PACK_AHEAD][8], valid[PACK_AHEAD];
+        // contiguous elements come from the one or two aligned 16 bytes that hold a group's
+        const uint32_t shift = k.si == 1 ? (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u : 0;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const uint32_t lo = i + 2 * q < k.inner ? src[2 * q * k.si] : 0;
-            const uint32_t hi = i + 2 * q + 1 < k.inner ? src[(2 * q + 1) * k.si] : 0;
-            w[q] = lo | (hi << 16);
+        for (uint32_t a = 0; a < PACK_AHEAD; ++a) {
+            const uint64_t i = i0 + a * 256;
+            valid[a] = (uint32_t)min((uint64_t)8, i < k.inner ? k.inner - i : 0);
+            uint4 x = make_uint4(0, 0, 0, 0), y = x;
+            if (k.si == 1) {
+                const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row + i) - shift);
+                if (valid[a]) x = from[0];
+                if (shift + 2 * valid[a] > 16) y = from[1];
+            } else {
+                uint32_t w[4];
+#pragma unroll
+                for (uint32_t q = 0; q < 4; ++q) {
+                    const uint16_t* at = row + (int64_t)(i + 2 * q) * k.si;
+                    w[q] = (2 * q < valid[a] ? (uint32_t)at[0] : 0u) | (2 * q + 1 < valid[a] ? (uint32_t)at[k.si] << 16 : 0u);
+                }
+                x = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            v[a][0] = x.x, v[a][1] = x.y, v[a][2] = x.z, v[a][3] = x.w;
+            v[a][4] = y.x, v[a][5] = y.y, v[a][6] = y.z, v[a][7] = y.w;
         }
-        store_words(k.dst + o * k.ld + i, w);
+#pragma unroll
+        for (uint32_t a = 0; a < PACK_AHEAD; ++a) {
+#pragma unroll
+            for (int s = 2; s; s >>= 1)
+                if (shift >> 2 & s) {
+#pragma unroll
+                    for (int q = 0; q + s < 8; ++q) v[a][q] = v[a][q + s];
+                }
+            uint32_t w[4];
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) {
+                w[q] = shift & 2 ? __funnelshift_r(v[a][q], v[a][q + 1], 16) : v[a][q];
+                if (valid[a] < 2 * q + 2) w[q] = valid[a] > 2 * q ? w[q] & 0xFFFFu : 0;
+            }
+            if (i0 + a * 256 < k.ld) store_words(to + i0 + a * 256, w);
+        }
     }
 }
 
@@ -1093,6 +1131,10 @@ struct Operand {
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// Rows of scratch matrices: whole lines of 128 bytes, which is what a row of a tensor copy's box reads (with rows a
+// multiple of 16 bytes apart that read takes two).
+static uint64_t padded(uint64_t elements) { return round_up(elements, 64); }
+
 // One call's scratch memory: laid out first, then allocated at once, and the operands' copies made in one launch.
 struct Scratch {
     cudaStream_t st;
@@ -1117,8 +1159,7 @@ struct Scratch {
         if (bytes) buf.alloc(bytes);
         if (!packs.count) return;
         for (uint32_t c = 0; c < packs.count; ++c) packs.of[c].dst = at<uint16_t>((int64_t)pack_at[c]);
-        const uint64_t groups = packs.of[packs.count - 1].end;
-        const unsigned grid = (unsigned)std::min<uint64_t>((groups + 255) / 256, 148 * 16);
+        const unsigned grid = (unsigned)std::min<uint64_t>((packs.of[packs.count - 1].end + 7) / 8, 148 * 32);
         launch_overlapped(pack_kernel, dim3(grid), 256, 0, dim3(0), st, packs);
     }
     // The operand as the tensor copies can read it: as it lies (K-major, or MN-major where allowed), or a copy.
@@ -1134,10 +1175,10 @@ struct Scratch {
         }
         // packed along the contiguous index, so that the copy reads and writes neighbouring elements
         const bool mn = allow_mn && o.rs == 1 && o.ks != 1;
-        const uint64_t outer = mn ? o.red : o.rows, inner = mn ? o.rows : o.red, ld = round_up(inner, 8);
+        const uint64_t outer = mn ? o.red : o.rows, inner = mn ? o.rows : o.red, ld = padded(inner);
         const uint32_t c = packs.count++;
         packs.of[c] = {static_cast<const uint16_t*>(o.p), mn ? o.ks : o.rs, mn ? o.rs : o.ks, outer, inner, ld, nullptr,
-                       (c ? packs.of[c - 1].end : 0) + outer * (ld / 8)};
+                       (c ? packs.of[c - 1].end : 0) + outer * ((ld / 8 + PACK_GROUPS - 1) / PACK_GROUPS)};
         o.at = reserve(outer * ld * 2);
         pack_at[c] = (uint64_t)o.at;
         o.mn = mn;
@@ -1433,7 +1474,7 @@ static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
     const bool write = products && (act || !fits(dy)), sum = mn && a.db.data;
     // clusters of up to 8 blocks, one below the other, as many as spread over the device; at least 16 rows a block,
     // and up to 128 rows a block no second cluster, nor the launch that joins the clusters' sums
-    const uint64_t ld = round_up(a.n, 8), strips = (a.n + DZ_COLS - 1) / DZ_COLS, most = (a.m + DZ_ROWS - 1) / DZ_ROWS;
+    const uint64_t ld = padded(a.n), strips = (a.n + DZ_COLS - 1) / DZ_COLS, most = (a.m + DZ_ROWS - 1) / DZ_ROWS;
     uint32_t cluster = 1;
     while (cluster < DZ_CLUSTER && cluster * 2 <= most) cluster *= 2;
     uint64_t clusters = 1;
