@@ -296,10 +296,31 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
     return result;
 }
 
+// adamw_values(moments, blocks, device) -> (m, v): the values of 8-bit moments as BF16
+PyObject* adamw_values(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    if (!expect(count, 3, "adamw_values")) return nullptr;
+    return guarded([&]() -> PyObject* {
+        oztt_adamw_moments moments;
+        if (PyBytes_GET_SIZE(args[0]) != sizeof moments) throw std::runtime_error("adamw_values: a record of another size");
+        std::memcpy(&moments, PyBytes_AS_STRING(args[0]), sizeof moments);
+        const int64_t blocks = PyLong_AsLongLong(args[1]);
+        const int device = (int)PyLong_AsLong(args[2]);
+        const auto options = at::TensorOptions(at::kBFloat16).device(at::kCUDA, (c10::DeviceIndex)device);
+        const at::Tensor m = at::empty({blocks * OZTT_ADAMW_BLOCK}, options), v = at::empty_like(m);
+        void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+        call([&](char* err, size_t len) {
+            return oztt_adamw_values(device, &moments, (uint64_t)blocks, static_cast<uint16_t*>(m.data_ptr()),
+                                     static_cast<uint16_t*>(v.data_ptr()), stream, err, len);
+        });
+        return Py_BuildValue("(NN)", wrapped(m), wrapped(v));
+    });
+}
+
 PyMethodDef methods[] = {
     {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear)), METH_FASTCALL, nullptr},
     {"linear_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear_backward)), METH_FASTCALL, nullptr},
     {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(adamw_step)), METH_FASTCALL, nullptr},
+    {"adamw_values", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(adamw_values)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -8,7 +8,7 @@ import struct
 import numpy as np
 import torch
 
-from . import OK, _binding, _errbuf, _lib, _raise
+from . import _binding
 
 __all__ = ["AdamW"]
 
@@ -120,13 +120,7 @@ class AdamW:
         BF16 tensors with 8, which hold the values of the codes exactly."""
         if self.state_bits == 32:
             return self._m, self._v
-        m, v = (torch.empty(self.blocks * BLOCK, dtype=torch.bfloat16, device=self.device) for _ in range(2))
-        err = _errbuf()
-        rc = _lib().oztt_adamw_values(self.device.index, self._record, self.blocks, m.data_ptr(), v.data_ptr(),
-                                      torch.cuda.current_stream(self.device).cuda_stream, err, len(err))
-        if rc != OK:
-            _raise(rc, err.value)
-        return m, v
+        return _torch.adamw_values(self._record, self.blocks, self.device.index)
 
     def state_dict(self) -> dict:
         """What load_state_dict needs to go on from here: the number of steps, the moments as they are kept, and the
