@@ -1169,10 +1169,11 @@ struct Scratch {
         const bool base = o.at >= 0 || aligned16(o.p);
         if (o.ks == 1 && o.rs % 8 == 0 && o.rs >= (int64_t)o.red && base) return;
         if (o.red == 1) o.ks = (int64_t)round_up(o.rows, 8);
-        if (allow_mn && o.rs == 1 && o.ks % 8 == 0 && o.ks >= (int64_t)o.rows && base) {
+        if (allow_mn && (o.rs == 1 || o.rows == 1) && o.ks % 8 == 0 && o.ks >= (int64_t)o.rows && base) {
             o.mn = true;
             return;
         }
+        if (o.at >= 0) throw Error(OZTT_ERUNTIME, "linear: a scratch matrix that the tensor copies cannot read");
         // packed along the contiguous index, so that the copy reads and writes neighbouring elements
         const bool mn = allow_mn && o.rs == 1 && o.ks != 1;
         const uint64_t outer = mn ? o.red : o.rows, inner = mn ? o.rows : o.red, ld = padded(inner);
@@ -1321,7 +1322,7 @@ static int plan(Task* tasks, int count, Scratch& scratch) {
         if (few_rows(t)) continue;
         if (t.p.red) {
             scratch.settle(t.p, true);
-            scratch.settle(t.q, t.e.rows > 32);  // (narrower boxes have no MN-major form)
+            scratch.settle(t.q, t.e.rows > 32 || t.q.at >= 0);  // (dz is made after the copies, so never copied itself)
         } else {  // nothing is read: any valid address and stride for the tensor maps
             t.p.at = t.q.at = scratch.reserve(256);
             t.p.rs = t.q.rs = 8;
@@ -1342,7 +1343,7 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
     }
     if (count == 2 && tasks[1].p.red > tasks[0].p.red) std::swap(tasks[0], tasks[1]);  // the longest tiles first
     uint64_t rows = 0, pair_tiles = 0, tiles = 0, blocks = 0;
-    bool empty = false;
+    bool empty = false, narrow = true;  // boxes of less than 64 rows have no MN-major form
     for (int i = 0; i < count; ++i) {
         scratch.place(tasks[i].p);
         scratch.place(tasks[i].q);
@@ -1352,6 +1353,7 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
         tiles += ((e.rows + 127) / 128) * ((e.cols + 127) / 128);
         blocks = std::max(blocks, blocks_of(tasks[i]));
         empty = empty || tasks[i].p.red == 0;
+        narrow = narrow && !tasks[i].q.mn;
     }
     if (count == 1 && few_rows(tasks[0])) {
         const Task& t = tasks[0];
@@ -1371,9 +1373,9 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
     //   512x2048    4096     17.2     15.9     26.1
     if (!empty && rows > 128 && (pair_tiles >= 37 || (pair_tiles >= 24 && blocks <= 24)))
         count == 2 ? launch_pairs<HALF, 2, 256>(tasks, st) : launch_pairs<HALF, 1, 256>(tasks, st);
-    else if (rows <= 16)
+    else if (rows <= 16 && narrow)
         launch_tiles<HALF, 1, 16, 6, 2>(tasks, st);
-    else if (rows <= 32)
+    else if (rows <= 32 && narrow)
         launch_tiles<HALF, 1, 32, 5, 2>(tasks, st);
     else if (rows <= 64 || tiles <= 32 || blocks <= 24)
         count == 2 ? launch_tiles<HALF, 2, 64, 4, 2>(tasks, st) : launch_tiles<HALF, 1, 64, 4, 2>(tasks, st);

@@ -134,6 +134,16 @@ def test_backward_few_rows(oztt, cuda, m):
     check_backward(oztt, dy, x, w, None, "none")
 
 
+@pytest.mark.parametrize("n", [1, 2, 7, 8, 16, 17, 24, 32, 33])
+@pytest.mark.parametrize("m", [1, 2, 9, 70, 300])
+def test_backward_narrow(oztt, cuda, m, n):
+    """Few output features: dz is a scratch matrix with as few columns, read across its rows for dw."""
+    for k in (8, 1, 200):
+        x, w, b, dy = make(m, n, k, torch.bfloat16, seed=m + n)
+        check_backward(oztt, dy, x, w, dy.roll(1, 0), "silu")
+        check_backward(oztt, dy, x, w, None, "none")
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_forward_activations(oztt, cuda, act, dtype):
