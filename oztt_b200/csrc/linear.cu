@@ -896,6 +896,56 @@ __global__ void __launch_bounds__(256)
     }
 }
 
+// ---- few terms -----------------------------------------------------------------------------------
+// out[i][j] = the sum of up to T products, for dw of a few tokens: bound by the bytes of the output, which the tiles of the
+// tensor cores finish no faster than 2.5 TB/s. A warp keeps 256 columns of P (8 a lane, contiguous) in registers and
+// walks down 8 or 16 rows, one 16-byte store a lane and row, the terms' factors of a row read from shared memory. 4480 x 8576
+// from 2, 4 and 8 terms: 12.5, 13.2 and 24 us (a fill of the same 77 MB: 20), by tiles 33 to 36.
+template <int T>
+constexpr uint32_t TERM_ROWS = T > 4 ? 16 : 8;
+template <bool HALF, int T>
+__global__ void __launch_bounds__(256)
+    few_terms_kernel(const uint16_t* __restrict__ p, int64_t p_term, const uint16_t* __restrict__ q, int64_t q_row,
+                     int64_t q_term, const uint32_t red, View out, uint64_t rows, uint64_t cols) {
+    constexpr uint32_t ROWS = TERM_ROWS<T>;
+    __shared__ __align__(16) f32x2 factors[8 * ROWS][T];  // of the block's rows, each twice
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t j = blockIdx.x * 256ull + lane * 8, i0 = blockIdx.y * (8ull * ROWS);
+    overlap_launches();
+    for (uint32_t k = threadIdx.x; k < 8 * ROWS * T; k += 256) {
+        const uint32_t r = k % (8 * ROWS), t = k / (8 * ROWS);
+        const float a = t < red && i0 + r < rows ? to_f32<HALF>(q[(int64_t)(i0 + r) * q_row + t * q_term]) : 0.0f;
+        factors[r][t] = splat2(a);
+    }
+    f32x2 x[T][4];
+#pragma unroll
+    for (uint32_t t = 0; t < T; ++t) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (t < red && j < cols) load_words(p + t * p_term + j, w);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[t][c] = unpack<HALF>(w[c]);
+    }
+    __syncthreads();
+    const uint32_t r0 = warp * ROWS;
+    if (j >= cols || i0 + r0 >= rows) return;  // (cols is a multiple of 8)
+    const uint32_t count = (uint32_t)min((uint64_t)ROWS, rows - i0 - r0);
+    uint16_t* to = element(out, i0 + r0, j);
+#pragma unroll 2
+    for (uint32_t r = 0; r < count; ++r) {
+        f32x2 sum[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t t = 0; t < T; ++t) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] = fma2(factors[r0 + r][t], x[t][c], sum[c]);
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[c] = pack<HALF>(sum[c]);
+        store_words(to, w);
+        to += out.rs;
+    }
+}
+
 // ---- passes over memory --------------------------------------------------------------------------
 
 // Copies of operands whose base or rows do not start on 16 bytes, which the tensor copies cannot read:
@@ -1239,6 +1289,27 @@ static Products<COUNT> describe_all(const Task* tasks, uint32_t tile_p, uint32_t
     return ps;
 }
 
+// How many clusters of `size` blocks of a kernel the device runs at once, a block to an SM (asked once).
+template <class Kernel>
+static uint32_t room_for(Kernel* kernel, uint32_t smem, uint32_t size, std::atomic<int>& known) {
+    int n = known.load();
+    if (!n) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(size);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = size;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        OZTT_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+        known.store(n > 0 ? n : -1);
+    }
+    return n > 0 ? (uint32_t)n : 0;
+}
+
 template <bool HALF, int COUNT, int BQ, int STAGES, int CTAS>
 static void launch_tiles(const Task* tasks, cudaStream_t st) {
     constexpr uint32_t SMEM = STAGES * (P_BYTES + BQ * BK * 2) + 256 + 1024;
@@ -1246,12 +1317,20 @@ static void launch_tiles(const Task* tasks, cudaStream_t st) {
     auto* kernel = product_kernel<HALF, COUNT, BQ, STAGES, CTAS>;
     allow_smem(kernel, SMEM, allowed, true);
     const Products<COUNT> ps = describe_all<HALF, COUNT>(tasks, BP, BQ, BQ);
-    // With few tiles the reduction is shared by up to 8 CTAs, as long as the CTAs are resident at once and each keeps at
-    // least two blocks of it; by 16 where that takes one CTA an SM at most, since few clusters of 16 find room in the
-    // device's parts at once (16 x 512 x 16384: 12.4 us with 8, 8.7 with 16; 128 x 1024 x 4096: 8.7 and 13.9).
+    // With few tiles the reduction is shared by a cluster of CTAs, each with at least two blocks of it: by as many, up to
+    // 8, as let all clusters find room in the device's parts at once, two CTAs to an SM (5 x 4480 x 8576, 35 tiles: 17.0 us
+    // with 6, 23.6 with 8 in two turns); by 16 where they do with a CTA to an SM (16 x 512 x 16384: 8.7 us, 12.4 with 8;
+    // 128 x 1024 x 4096, where they do not: 13.9 and 8.7).
+    static_assert(CTAS == 2, "the room below is that of two CTAs to an SM");
     const uint32_t shortest = std::min(ps.of[0].num_kb, ps.of[COUNT - 1].num_kb);
+    static std::atomic<int> known[MAX_SPLIT + 1];
+    const auto alone = [&](uint32_t size) { return room_for(kernel, SMEM, size, known[size]); };
     uint32_t split = 1;
-    while (split < MAX_SPLIT && ps.tiles * split * 2 <= (split < 8 ? 148 * CTAS : 148) && shortest / (split * 2) >= 2) split *= 2;
+    if (shortest / MAX_SPLIT >= 2 && ps.tiles * MAX_SPLIT <= 148 && ps.tiles <= alone(MAX_SPLIT))
+        split = MAX_SPLIT;
+    else
+        for (uint32_t s = std::min<uint32_t>(8, shortest / 2); s > 1 && split == 1; --s)
+            if (ps.tiles * s <= 296 && ps.tiles <= std::max(2 * alone(s), alone((s + 1) / 2))) split = s;
     launch_overlapped(kernel, dim3(ps.tiles * split), THREADS, SMEM, dim3(split), st, ps, error_word());
 }
 
@@ -1285,6 +1364,12 @@ static bool takes_vectors(const Task& t) {
 static bool few_rows(const Task& t) {
     return t.p.red && t.p.ks == 1 && t.q.ks == 1 && (t.e.rows == 1 || (t.e.rows <= 4 && !takes_vectors(t)));
 }
+// A sum of up to 8 terms without an epilogue, over columns that P has side by side, goes to the kernel for those.
+static bool few_terms(const Task& t) {
+    const Epilogue& e = t.e;
+    return t.p.red && t.p.red <= 8 && t.p.mn && e.vec == 8 && e.cols % 8 == 0 && e.rows <= 65535 * 64 &&
+           e.act == OZTT_ACT_NONE && !e.bias && !e.pre.p && !e.res.p;
+}
 static uint64_t blocks_of(const Task& t) { return (t.p.red + BK - 1) / BK; }
 static uint64_t pair_tiles_of(const Task& t) { return ((t.e.rows + 255) / 256) * ((t.e.cols + 255) / 256); }
 // Two products share a launch, and its tiles' size, where one launch less counts or their tiles fill up one another's
@@ -1296,6 +1381,23 @@ static bool together(const Task* tasks, int count) {
     if (count < 2 || std::min(tasks[0].e.rows, tasks[1].e.rows) <= 64) return false;
     const uint64_t b0 = blocks_of(tasks[0]), b1 = blocks_of(tasks[1]), t0 = pair_tiles_of(tasks[0]), t1 = pair_tiles_of(tasks[1]);
     return std::max(b0, b1) <= 24 || (t0 + t1 <= 148 && t0 * b0 + t1 * b1 >= 52 * std::max(b0, b1));
+}
+
+template <bool HALF>
+static void launch_few_terms(const Task& t, cudaStream_t st) {
+    const auto go = [&](auto* kernel, uint32_t block_rows) {
+        const dim3 grid((unsigned)((t.e.cols + 255) / 256), (unsigned)((t.e.rows + block_rows - 1) / block_rows));
+        launch_overlapped(kernel, grid, 256, 0, dim3(0), st, static_cast<const uint16_t*>(t.p.p), t.p.ks,
+                          static_cast<const uint16_t*>(t.q.p), t.q.rs, t.q.ks, (uint32_t)t.p.red, t.e.out, t.e.rows, t.e.cols);
+    };
+    if (t.p.red == 1)
+        go(few_terms_kernel<HALF, 1>, 8 * TERM_ROWS<1>);
+    else if (t.p.red == 2)
+        go(few_terms_kernel<HALF, 2>, 8 * TERM_ROWS<2>);
+    else if (t.p.red <= 4)
+        go(few_terms_kernel<HALF, 4>, 8 * TERM_ROWS<4>);
+    else
+        go(few_terms_kernel<HALF, 8>, 8 * TERM_ROWS<8>);
 }
 
 // The products of one call, out = epilogue(Q P^T), p the operand of the output's columns and q of its rows: what
@@ -1363,6 +1465,7 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
                                     : launch_few<HALF, 4, false>;
         return go(t, st);
     }
+    if (count == 1 && few_terms(tasks[0])) return launch_few_terms<HALF>(tasks[0], st);
     // Which tiles, by what was measured (us, BF16, single products):
     //   output      sum    64 rows  128 rows  pairs
     //   512x4096    1024     12.1     13.3     11.5      pairs from half the device's SMs on, and from a third where

@@ -134,6 +134,16 @@ def test_backward_few_rows(oztt, cuda, m):
     check_backward(oztt, dy, x, w, None, "none")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 6, 7, 8])
+def test_sums_of_few_terms(oztt, cuda, dtype, m):
+    for n, k in ((264, 520), (1, 8), (129, 1048)):
+        x, w, b, dy = make(m, n, k, dtype, seed=m)
+        check_backward(oztt, dy, x, w, None, "none")
+    x, w, b, r = make(203, 264, m, dtype, seed=m)
+    check_forward(oztt, x, w.t().contiguous().t(), None, None, "none")
+
+
 @pytest.mark.parametrize("n", [1, 2, 7, 8, 16, 17, 24, 32, 33])
 @pytest.mark.parametrize("m", [1, 2, 9, 70, 300])
 def test_backward_narrow(oztt, cuda, m, n):
