@@ -144,6 +144,14 @@ def test_sums_of_few_terms(oztt, cuda, dtype, m):
     check_forward(oztt, x, w.t().contiguous().t(), None, None, "none")
 
 
+@pytest.mark.parametrize("blocks", [3, 4, 6, 7, 9, 10, 12, 14, 31, 33])
+@pytest.mark.parametrize("m", [5, 30, 64, 200])
+def test_sums_shared_by_any_number(oztt, cuda, m, blocks):
+    """Sums of `blocks` stretches of 64 terms (the last one short), shared by 1 to 8 or by 16 blocks of the device."""
+    x, w, b, r = make(m, 200, 64 * blocks - 24, torch.bfloat16, seed=blocks)
+    check_forward(oztt, x, w, b, r, "relu", pre=True)
+
+
 @pytest.mark.parametrize("n", [1, 2, 7, 8, 16, 17, 24, 32, 33])
 @pytest.mark.parametrize("m", [1, 2, 9, 70, 300])
 def test_backward_narrow(oztt, cuda, m, n):
