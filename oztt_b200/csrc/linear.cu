@@ -52,7 +52,7 @@ struct Epilogue {
     const void* bias;                    // may be null
     int64_t bias_stride;
     int32_t act;                         // OZTT_ACT_*
-    int32_t vec;                         // columns that one access may take: 1, 4 or 8
+    int32_t vec;                         // columns that one access may take: 1, 4, 8 or 16
 };
 
 // ---- activations in 32 bits ----------------------------------------------------------------------
@@ -182,7 +182,7 @@ __device__ __forceinline__ uint32_t pack(f32x2 v) {
 
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
-// 16-bit values w.. by one access of 8 or 16 bytes.
+// 16-bit values w.. by one access of 8, 16 or (stores) 32 bytes.
 __device__ __forceinline__ void load_words(const uint16_t* p, uint32_t (&w)[2]) {
     const uint2 v = *reinterpret_cast<const uint2*>(p);
     w[0] = v.x, w[1] = v.y;
@@ -196,6 +196,11 @@ __device__ __forceinline__ void store_words(uint16_t* p, const uint32_t (&w)[2])
 }
 __device__ __forceinline__ void store_words(uint16_t* p, const uint32_t (&w)[4]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store_words(uint16_t* p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
 }
 
 // ---- the tile product ----------------------------------------------------------------------------
@@ -543,7 +548,13 @@ __global__ void __launch_bounds__(THREADS, CTAS)
 // tensor memory while the next tile accumulates in the other. Sixteen warps finish them (the latencies of the path
 // from tensor memory to the stores need so many), each 32 columns of a quarter of the rows: 8 rows at a time go
 // through a patch of shared memory of the warp's own, from which a lane takes 8 neighbouring columns of a row, so
-// that bias, activation, residual and stores run on 16-byte accesses.
+// that bias, activation, residual and stores run on 16-byte accesses. Bound by the tensor pipe where the sum is long, by
+// the stores where it is short.
+// TURNED, for outputs that take 32-byte accesses and have no residual: the operands change sides, a lane of tensor
+// memory is a row of the output and holds its neighbouring columns, which go to memory as they are, a whole sector a
+// lane and store. 8192 x 8192 x 64: 34.8 us, through patches 54.0 (a fill takes 35); 4096 x 4096 x 512 18.7 and 22.3;
+// 8192 x 4096 x 4096 188 and 192; with a residual, which a lane would read a sector at a time too, the patches are
+// faster: 8192 x 8192 x 256 82.9 us, turned 97.7.
 constexpr uint32_t PAIR_STAGES_BYTES = 196608;
 constexpr uint32_t FINISHERS = 16;
 constexpr uint32_t PAIR_THREADS = (2 + FINISHERS) * 32;  // warp 0 loads, warp 1 issues, the others finish
@@ -591,7 +602,7 @@ __device__ __forceinline__ const Product& tile_at(const Products<COUNT>& ps, uin
     return pr;
 }
 
-template <bool HALF, int COUNT, int BQ>
+template <bool HALF, int COUNT, int BQ, bool TURNED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     pair_product_kernel(const __grid_constant__ Products<COUNT> ps, int* err) {
     constexpr uint32_t HALF_Q = BQ / 2;
@@ -734,6 +745,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             uint32_t tp, tq;
             const Product& pr = tile_at(ps, tile, tp, tq);
             const Epilogue& e = pr.e;
+            if constexpr (TURNED) {  // 32 rows by a quarter of the tile's columns
+                const uint64_t i0 = (uint64_t)tp * 2 * BP + rank * BP + quarter * 32u, j0 = (uint64_t)tq * BQ + c0;
+                const uint32_t cols = i0 < e.rows && j0 < e.cols ? (uint32_t)min((uint64_t)ROWS, e.cols - j0) : 0;
+                const bool mine = i0 + lane < e.rows, has_bias = e.bias;
+                uint16_t* out = element(e.out, i0 + lane, j0);
+                uint16_t* pre = e.pre.p ? element(e.pre, i0 + lane, j0) : nullptr;
+                if (has_bias) {
+                    __syncwarp();  // the tile before has read its own
+#pragma unroll
+                    for (uint32_t c = 0; c < ROWS; c += 32) patch[c + lane] = bias_at<HALF>(e, j0 + c + lane);
+                    __syncwarp();
+                }
+                if (!mbar_wait(tfull_bar + acc, acc_phase, abort_flag, err, ERR_WAIT_EPILOGUE)) break;
+                tc_fence_after();
+                const uint32_t tbase = tmem_base + ((quarter * 32u) << 16) + acc * BQ + c0;
+#pragma unroll 1
+                for (uint32_t c = 0; c < cols; c += 16) {
+                    uint32_t v[16];
+                    __syncwarp();
+                    tmem_ld16(tbase + c, v);
+                    f32x2 z[8];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) z[q] = pk2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1]));
+                    if (has_bias) {
+                        const ulonglong2* b = reinterpret_cast<const ulonglong2*>(patch + c);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const ulonglong2 x = b[q];
+                            z[2 * q] = add2(z[2 * q], x.x), z[2 * q + 1] = add2(z[2 * q + 1], x.y);
+                        }
+                    }
+                    if (!mine) continue;
+                    if (c + 16 <= cols) {
+                        finish_vector<HALF, 8>(out + c, pre ? pre + c : nullptr, false, e.act, z, {});
+                    } else {
+                        float f[16];
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) unpk2(z[q], f[2 * q], f[2 * q + 1]);
+                        finish_scattered<HALF, 16>(Scattered(e, i0 + lane, j0 + c, 0, 1), cols - c, e.act, f);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_remote_relaxed(map_to(smem_u32(tempty_bar + acc), 0));
+                acc ^= 1u;
+                if (acc == 0) acc_phase ^= 1u;
+                continue;
+            }
             const uint64_t j0 = (uint64_t)tp * 2 * BP + rank * BP + quarter * 32u;
             const uint64_t i0 = (uint64_t)tq * BQ + c0;
             const bool vec = e.vec >= 8 && j0 + 32 <= e.cols;
@@ -1259,28 +1318,29 @@ struct Task {
 };
 
 template <bool HALF>
-static Product describe(const Task& t, uint32_t tile_p, uint32_t tile_q, uint32_t box_q) {
+static Product describe(const Task& t, uint32_t tile_p, uint32_t tile_q, uint32_t box_q, bool turned) {
     Product pr;
-    pr.p = operand_map(t.p, HALF, BP);
-    pr.q = operand_map(t.q, HALF, box_q);
+    const Operand &p = turned ? t.q : t.p, &q = turned ? t.p : t.q;
+    pr.p = operand_map(p, HALF, BP);
+    pr.q = operand_map(q, HALF, box_q);
     pr.e = t.e;
-    pr.tiles_p = (uint32_t)((t.e.cols + tile_p - 1) / tile_p);
-    pr.tiles_q = (uint32_t)((t.e.rows + tile_q - 1) / tile_q);
+    pr.tiles_p = (uint32_t)(((turned ? t.e.rows : t.e.cols) + tile_p - 1) / tile_p);
+    pr.tiles_q = (uint32_t)(((turned ? t.e.cols : t.e.rows) + tile_q - 1) / tile_q);
     pr.num_kb = (uint32_t)((t.p.red + BK - 1) / BK);
-    pr.p_mn = t.p.mn;
-    pr.q_mn = t.q.mn;
+    pr.p_mn = p.mn;
+    pr.q_mn = q.mn;
     // kind::f16: 32-bit sums, A and B of one type, their majors, N = tile_q, M = tile_p
     const uint32_t type = HALF ? 0u : 1u;
-    pr.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)t.p.mn << 15) | ((uint32_t)t.q.mn << 16) |
+    pr.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)p.mn << 15) | ((uint32_t)q.mn << 16) |
                ((tile_q >> 3) << 17) | ((tile_p >> 4) << 24);
     return pr;
 }
 template <bool HALF, int COUNT>
-static Products<COUNT> describe_all(const Task* tasks, uint32_t tile_p, uint32_t tile_q, uint32_t box_q) {
+static Products<COUNT> describe_all(const Task* tasks, uint32_t tile_p, uint32_t tile_q, uint32_t box_q, bool turned) {
     Products<COUNT> ps;
     uint64_t tiles = 0;
     for (int i = 0; i < COUNT; ++i) {
-        ps.of[i] = describe<HALF>(tasks[i], tile_p, tile_q, box_q);
+        ps.of[i] = describe<HALF>(tasks[i], tile_p, tile_q, box_q, turned);
         tiles += (uint64_t)ps.of[i].tiles_p * ps.of[i].tiles_q;
     }
     if (tiles >= (1ull << 28)) throw Error(OZTT_EINVAL, "linear: problem too large");
@@ -1316,7 +1376,7 @@ static void launch_tiles(const Task* tasks, cudaStream_t st) {
     static std::atomic<uint64_t> allowed{0};
     auto* kernel = product_kernel<HALF, COUNT, BQ, STAGES, CTAS>;
     allow_smem(kernel, SMEM, allowed, true);
-    const Products<COUNT> ps = describe_all<HALF, COUNT>(tasks, BP, BQ, BQ);
+    const Products<COUNT> ps = describe_all<HALF, COUNT>(tasks, BP, BQ, BQ, false);
     // With few tiles the reduction is shared by a cluster of CTAs, each with at least two blocks of it: by as many, up to
     // 8, as let all clusters find room in the device's parts at once, two CTAs to an SM (5 x 4480 x 8576, 35 tiles: 17.0 us
     // with 6, 23.6 with 8 in two turns); by 16 where they do with a CTA to an SM (16 x 512 x 16384: 8.7 us, 12.4 with 8;
@@ -1334,13 +1394,13 @@ static void launch_tiles(const Task* tasks, cudaStream_t st) {
     launch_overlapped(kernel, dim3(ps.tiles * split), THREADS, SMEM, dim3(split), st, ps, error_word());
 }
 
-template <bool HALF, int COUNT, int BQ>
+template <bool HALF, int COUNT, int BQ, bool TURNED>
 static void launch_pairs(const Task* tasks, cudaStream_t st) {
     constexpr uint32_t SMEM = PAIR_STAGES_BYTES + FINISHERS * PATCH_BYTES + 256 + 1024;
     static std::atomic<uint64_t> allowed{0};
-    auto* kernel = pair_product_kernel<HALF, COUNT, BQ>;
+    auto* kernel = pair_product_kernel<HALF, COUNT, BQ, TURNED>;
     allow_smem(kernel, SMEM, allowed);
-    const Products<COUNT> ps = describe_all<HALF, COUNT>(tasks, 2 * BP, BQ, BQ / 2);
+    const Products<COUNT> ps = describe_all<HALF, COUNT>(tasks, 2 * BP, BQ, BQ / 2, TURNED);
     launch_overlapped(kernel, dim3(2 * std::min<uint32_t>(ps.tiles, 74)), PAIR_THREADS, SMEM, dim3(0), st, ps, error_word());
 }
 
@@ -1367,7 +1427,7 @@ static bool few_rows(const Task& t) {
 // A sum of up to 8 terms without an epilogue, over columns that P has side by side, goes to the kernel for those.
 static bool few_terms(const Task& t) {
     const Epilogue& e = t.e;
-    return t.p.red && t.p.red <= 8 && t.p.mn && e.vec == 8 && e.cols % 8 == 0 && e.rows <= 65535 * 64 &&
+    return t.p.red && t.p.red <= 8 && t.p.mn && e.vec >= 8 && e.cols % 8 == 0 && e.rows <= 65535 * 64 &&
            e.act == OZTT_ACT_NONE && !e.bias && !e.pre.p && !e.res.p;
 }
 static uint64_t blocks_of(const Task& t) { return (t.p.red + BK - 1) / BK; }
@@ -1416,7 +1476,7 @@ static int plan(Task* tasks, int count, Scratch& scratch) {
             };
             return fits(e.out) && fits(e.pre) && fits(e.res);
         };
-        e.vec = takes(8) ? 8 : takes(4) ? 4 : 1;
+        e.vec = takes(16) ? 16 : takes(8) ? 8 : takes(4) ? 4 : 1;
         tasks[live++] = t;
     }
     for (int i = 0; i < live; ++i) {
@@ -1445,7 +1505,7 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
     }
     if (count == 2 && tasks[1].p.red > tasks[0].p.red) std::swap(tasks[0], tasks[1]);  // the longest tiles first
     uint64_t rows = 0, pair_tiles = 0, tiles = 0, blocks = 0;
-    bool empty = false, narrow = true;  // boxes of less than 64 rows have no MN-major form
+    bool empty = false, wide = true, narrow = true;  // boxes of less than 64 rows have no MN-major form
     for (int i = 0; i < count; ++i) {
         scratch.place(tasks[i].p);
         scratch.place(tasks[i].q);
@@ -1455,6 +1515,7 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
         tiles += ((e.rows + 127) / 128) * ((e.cols + 127) / 128);
         blocks = std::max(blocks, blocks_of(tasks[i]));
         empty = empty || tasks[i].p.red == 0;
+        wide = wide && e.vec >= 16 && !e.res.p;
         narrow = narrow && !tasks[i].q.mn;
     }
     if (count == 1 && few_rows(tasks[0])) {
@@ -1474,9 +1535,12 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
     //   512x2048    1024      9.8     10.5     11.2      64 rows where 128 would leave most SMs idle or the sum is
     //   256x2048    4096     12.0     13.7     25.6      short, since the CTAs of a split sum join sooner
     //   512x2048    4096     17.2     15.9     26.1
-    if (!empty && rows > 128 && (pair_tiles >= 37 || (pair_tiles >= 24 && blocks <= 24)))
-        count == 2 ? launch_pairs<HALF, 2, 256>(tasks, st) : launch_pairs<HALF, 1, 256>(tasks, st);
-    else if (rows <= 16 && narrow)
+    if (!empty && rows > 128 && (pair_tiles >= 37 || (pair_tiles >= 24 && blocks <= 24))) {
+        if (wide)
+            count == 2 ? launch_pairs<HALF, 2, 256, true>(tasks, st) : launch_pairs<HALF, 1, 256, true>(tasks, st);
+        else
+            count == 2 ? launch_pairs<HALF, 2, 256, false>(tasks, st) : launch_pairs<HALF, 1, 256, false>(tasks, st);
+    } else if (rows <= 16 && narrow)
         launch_tiles<HALF, 1, 16, 6, 2>(tasks, st);
     else if (rows <= 32 && narrow)
         launch_tiles<HALF, 1, 32, 5, 2>(tasks, st);

@@ -9,6 +9,7 @@ products.
 """
 
 import math
+import struct
 
 import pytest
 import torch
@@ -150,6 +151,34 @@ def test_sums_shared_by_any_number(oztt, cuda, m, blocks):
     """Sums of `blocks` stretches of 64 terms (the last one short), shared by 1 to 8 or by 16 blocks of the device."""
     x, w, b, r = make(m, 200, 64 * blocks - 24, torch.bfloat16, seed=blocks)
     check_forward(oztt, x, w, b, r, "relu", pre=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m,n,k", [(1700, 2096, 40), (2049, 1536, 264), (1531, 2064, 1096)])
+def test_forward_large_without_residual(oztt, cuda, dtype, act, m, n, k):
+    x, w, b, r = make(m, n, k, dtype, seed=k)
+    check_forward(oztt, x, w, b, None, act, pre=act != "relu")
+    check_forward(oztt, x, w.t().contiguous().t(), None, None, act)
+
+
+@pytest.mark.parametrize("n", [2064, 2065, 2079, 2090])
+@pytest.mark.parametrize("offset", [0, 8, 16])
+def test_outputs_inside_wider_ones(oztt, cuda, n, offset):
+    """y and pre as columns of wider matrices, through the C ABI: their values, and nothing beside them written."""
+    m, k, ld, dt = 1700, 136, 2112, torch.bfloat16
+    x, w, b, _ = make(m, n, k, dt, seed=n)
+    bufs = [torch.full((m, ld), 7.0, dtype=dt, device="cuda") for _ in range(2)]
+    y, pre = (t[:, offset:offset + n] for t in bufs)
+    views = [(t.data_ptr(), t.stride(0), t.stride(1)) for t in (x, w)] + [(b.data_ptr(), 0, 1), (0, 0, 0)]
+    views += [(t.data_ptr(), ld, 1) for t in (y, pre)]
+    args = struct.pack("=ii3Q" + 6 * "Qqq", 0, 0, m, n, k, *(v for view in views for v in view))
+    oztt.call("oztt_linear_forward", 0, args, torch.cuda.current_stream().cuda_stream)
+    want = x.double() @ w.double().t() + b.double()
+    err = (k + 2) * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t() + b.double().abs())
+    for t, whole in ((y, bufs[0]), (pre, bufs[1])):
+        within(t, want, U[dt] * want.abs() + (1 + U[dt]) * err + TINY[dt], "y and pre")
+        assert bool((whole[:, :offset] == 7).all()) and bool((whole[:, offset + n:] == 7).all())
 
 
 @pytest.mark.parametrize("n", [1, 2, 7, 8, 16, 17, 24, 32, 33])
