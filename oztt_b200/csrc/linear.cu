@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
 // the stores where it is short.
 // TURNED, for outputs that take 32-byte accesses and have no residual: the operands change sides, a lane of tensor
 // memory is a row of the output and holds its neighbouring columns, which go to memory as they are, a whole sector a
-// lane and store. 8192 x 8192 x 64: 34.8 us, through patches 54.0 (a fill takes 35); 4096 x 4096 x 512 18.7 and 22.3;
+// lane and store. 8192 x 8192 x 64: 34.8 us, through patches 54.0 (stores alone 18); 4096 x 4096 x 512 18.7 and 22.3;
 // 8192 x 4096 x 4096 188 and 192; with a residual, which a lane would read a sector at a time too, the patches are
 // faster: 8192 x 8192 x 256 82.9 us, turned 97.7.
 constexpr uint32_t PAIR_STAGES_BYTES = 196608;
@@ -956,10 +956,12 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---- few terms -----------------------------------------------------------------------------------
-// out[i][j] = the sum of up to T products, for dw of a few tokens: bound by the bytes of the output, which the tiles of the
-// tensor cores finish no faster than 2.5 TB/s. A warp keeps 256 columns of P (8 a lane, contiguous) in registers and
-// walks down 8 or 16 rows, one 16-byte store a lane and row, the terms' factors of a row read from shared memory. 4480 x 8576
-// from 2, 4 and 8 terms: 12.5, 13.2 and 24 us (a fill of the same 77 MB: 20), by tiles 33 to 36.
+// out[i][j] = the sum of up to T products, for dw of a few tokens, whose output the tiles of the tensor cores finish at
+// 3.9 TB/s at most. Up to 4 terms are bound by the stores, more by the products on the 32-bit pipe. A warp keeps 256
+// columns of P (8 a lane, contiguous) in registers and walks down 8 or 16 rows, one 16-byte store a lane and row, the
+// terms' factors of a row read from shared memory. 4480 x 8576 from 2, 4 and 8 terms: 12.3, 12.3 and 21.7 us (stores alone
+// 10.6, at 7.3 TB/s), by tiles 24; 1024 x 1024 2.2, 2.3 and 3.9, by tiles 6.7; 8192 x 8192 from 8 38.9, by tiles 35. 8 terms
+// with 8 rows a warp: 24.9; with 4 columns a lane 23.9.
 template <int T>
 constexpr uint32_t TERM_ROWS = T > 4 ? 16 : 8;
 template <bool HALF, int T>
@@ -967,14 +969,14 @@ __global__ void __launch_bounds__(256)
     few_terms_kernel(const uint16_t* __restrict__ p, int64_t p_term, const uint16_t* __restrict__ q, int64_t q_row,
                      int64_t q_term, const uint32_t red, View out, uint64_t rows, uint64_t cols) {
     constexpr uint32_t ROWS = TERM_ROWS<T>;
-    __shared__ __align__(16) f32x2 factors[8 * ROWS][T];  // of the block's rows, each twice
+    __shared__ __align__(16) float factors[8 * ROWS][T];  // of the block's rows
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint64_t j = blockIdx.x * 256ull + lane * 8, i0 = blockIdx.y * (8ull * ROWS);
     overlap_launches();
     for (uint32_t k = threadIdx.x; k < 8 * ROWS * T; k += 256) {
         const uint32_t r = k % (8 * ROWS), t = k / (8 * ROWS);
         const float a = t < red && i0 + r < rows ? to_f32<HALF>(q[(int64_t)(i0 + r) * q_row + t * q_term]) : 0.0f;
-        factors[r][t] = splat2(a);
+        factors[r][t] = a;
     }
     f32x2 x[T][4];
 #pragma unroll
@@ -994,8 +996,9 @@ __global__ void __launch_bounds__(256)
         f32x2 sum[4] = {0, 0, 0, 0};
 #pragma unroll
         for (uint32_t t = 0; t < T; ++t) {
+            const f32x2 a = splat2(factors[r0 + r][t]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) sum[c] = fma2(factors[r0 + r][t], x[t][c], sum[c]);
+            for (int c = 0; c < 4; ++c) sum[c] = fma2(a, x[t][c], sum[c]);
         }
         uint32_t w[4];
 #pragma unroll
