@@ -1,0 +1,38 @@
+"""Orderings that the kernels' sources have to state, since no result shows for certain that one is missing."""
+
+import re
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parent.parent / "oztt_b200" / "csrc"
+SOURCES = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh"))
+
+
+def without_comments(path):
+    return re.sub(r"//[^\n]*|/\*.*?\*/", "", path.read_text(), flags=re.S)
+
+
+def statements(text):
+    """The asm statements of a source, whole."""
+    for at in re.finditer(r"\basm\b(?:\s+volatile)?\s*\(", text):
+        depth, end = 1, at.end()
+        while depth:
+            depth += {"(": 1, ")": -1}.get(text[end], 0)
+            end += 1
+        yield text[at.start():end]
+
+
+@pytest.mark.parametrize("path", SOURCES, ids=lambda p: p.name)
+def test_loads_from_tensor_memory_are_waited_for(path):
+    """A load from tensor memory writes its registers until tcgen05.wait::ld: the wait names every one of them as its
+    own, in the same function and behind the load, or the compiler may use one before it."""
+    asm = list(statements(without_comments(path)))
+    loads = [i for i, s in enumerate(asm) if "tcgen05.ld." in s]
+    for i in loads:
+        regs = re.findall(r'"=r"\((\w+\[\d+\])\)', asm[i])
+        assert len(regs) == int(re.search(r"\.x(\d+)\.b32", asm[i]).group(1))
+        wait = asm[i] if "tcgen05.wait::ld" in asm[i] else asm[i + 1]
+        assert "tcgen05.wait::ld" in wait
+        assert wait is asm[i] or re.findall(r'"\+r"\((\w+\[\d+\])\)', wait) == regs, asm[i][:80]
+    assert len([s for s in asm if "tcgen05.wait::ld" in s]) == len(loads)
