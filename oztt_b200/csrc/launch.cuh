@@ -34,7 +34,8 @@ struct DeviceScope {
 };
 
 // Lets the next kernel of the stream start while this one ends, and waits for the one before, which must be over
-// before anything in memory is read or written (both do nothing where the launch did not ask for the overlap).
+// before anything in memory is read or written (both do nothing where the launch did not ask for the overlap). The
+// kernel before may still be writing what this one reads, so no input of such a kernel is `const __restrict__`.
 __device__ __forceinline__ void overlap_launches() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -876,7 +876,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 constexpr int FEW_COLS = 4;  // output columns (rows of P) of a warp
 template <bool HALF, int M, bool VEC>
 __global__ void __launch_bounds__(256)
-    few_rows_kernel(const uint16_t* __restrict__ p, int64_t ldp, const uint16_t* __restrict__ q, int64_t ldq,
+    few_rows_kernel(const uint16_t* p, int64_t ldp, const uint16_t* q, int64_t ldq,
                     const uint32_t red, const __grid_constant__ Epilogue e) {
     __shared__ float sums[8][FEW_COLS * M];
     constexpr uint32_t STEP = VEC ? 256 : 32;  // reduction elements of a warp's access
@@ -966,7 +966,7 @@ template <int T>
 constexpr uint32_t TERM_ROWS = T > 4 ? 16 : 8;
 template <bool HALF, int T>
 __global__ void __launch_bounds__(256)
-    few_terms_kernel(const uint16_t* __restrict__ p, int64_t p_term, const uint16_t* __restrict__ q, int64_t q_row,
+    few_terms_kernel(const uint16_t* p, int64_t p_term, const uint16_t* q, int64_t q_row,
                      int64_t q_term, const uint32_t red, View out, uint64_t rows, uint64_t cols) {
     constexpr uint32_t ROWS = TERM_ROWS<T>;
     __shared__ __align__(16) float factors[8 * ROWS][T];  // of the block's rows
@@ -1189,7 +1189,7 @@ __global__ void __launch_bounds__(256, !VEC ? 3 : ACT == OZTT_ACT_NONE ? 8 : 4)
 
 // db from the clusters' sums: a block takes 32 columns, each warp every eighth cluster.
 template <bool HALF>
-__global__ void __launch_bounds__(256) db_kernel(const float* __restrict__ partial, uint64_t clusters, uint64_t n,
+__global__ void __launch_bounds__(256) db_kernel(const float* partial, uint64_t clusters, uint64_t n,
                                                  uint16_t* __restrict__ db, int64_t stride) {
     __shared__ float sums[8][32];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

@@ -36,3 +36,16 @@ def test_loads_from_tensor_memory_are_waited_for(path):
         assert "tcgen05.wait::ld" in wait
         assert wait is asm[i] or re.findall(r'"\+r"\((\w+\[\d+\])\)', wait) == regs, asm[i][:80]
     assert len([s for s in asm if "tcgen05.wait::ld" in s]) == len(loads)
+
+
+@pytest.mark.parametrize("path", SOURCES, ids=lambda p: p.name)
+def test_overlapped_kernels_do_not_call_their_inputs_constant(path):
+    """A kernel that starts while the one before it ends (overlap_launches) may read what that one is still writing: its
+    inputs do change while it runs, so none is `const __restrict__`, which would let loads move ahead of its wait or
+    take the path of data that nobody writes."""
+    text = without_comments(path)
+    for at in re.finditer(r"__global__", text):
+        end = text.index("{", at.start())
+        body = text[end:text.index("\n}", end)]
+        if "overlap_launches" in body:
+            assert not re.search(r"\bconst\s+\w+\s*\*\s*__restrict__", text[at.start():end])
