@@ -333,7 +333,10 @@ __device__ __forceinline__ void chunk(const Tensor& t, uint64_t first, uint32_t 
         }
         if (P32) {
             store(wide_words(p), source, i, n, whole);
-            if (ptype != OZTT_TYPE_FP32) store(half_words(p, ptype), t.param, i, n, whole);
+            if (ptype != OZTT_TYPE_FP32)
+                store(half_words(p, ptype), t.param, i, n, whole);
+            else if (t.master)  // an FP32 parameter beside its master: the same value
+                store(wide_words(p), t.param, i, n, whole);
         } else {
             store(half_words(p, ptype), t.param, i, n, whole);
         }
