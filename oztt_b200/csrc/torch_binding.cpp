@@ -8,6 +8,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -105,6 +106,14 @@ bool wants_gradient(std::initializer_list<const at::Tensor*> all) {
     return false;
 }
 
+// A tangent of torch's forward mode would be lost without a trace: the products have no derivatives of that kind.
+void refuse_tangents(const char* who, std::initializer_list<const at::Tensor*> all) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const at::Tensor* t : all)
+        if (t && t->_fw_grad(0).defined())
+            throw std::runtime_error(std::string(who) + ": forward-mode differentiation is not supported");
+}
+
 PyObject* wrapped(const at::Tensor& t) {
     if (t.defined()) return THPVariable_Wrap(t);
     Py_RETURN_NONE;
@@ -144,7 +153,10 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
         }
         if (r && !(fits && r->size(dim - 1) == n))
             refuse("linear: residual " + text(*r) + " does not match the output of x " + text(x) + " and weight " + text(w));
-        if (args[6] == Py_True && wants_gradient({&x, &w, b, r})) Py_RETURN_NONE;
+        if (args[6] == Py_True) {
+            refuse_tangents(who, {&x, &w, b, r});
+            if (wants_gradient({&x, &w, b, r})) Py_RETURN_NONE;
+        }
         at::NoGradGuard no_grad;
         const at::Tensor x2 = rows_of(x, m, k);
         const at::Tensor r2 = r ? rows_of(*r, m, n) : at::Tensor();
@@ -199,6 +211,7 @@ PyObject* linear_backward(PyObject*, PyObject* const* args, Py_ssize_t count) {
         if (a.activation != OZTT_ACT_NONE && !pre) refuse("linear_backward: the activation needs pre");
         if (pre && pre->sizes() != dy.sizes())
             refuse("linear_backward: pre " + text(*pre) + " does not match dy " + text(dy));
+        refuse_tangents(who, {&dy, &x, &w, pre});
         at::NoGradGuard no_grad;
         const at::Tensor x2 = rows_of(x, m, k), dy2 = rows_of(dy, m, n), pre2 = pre ? rows_of(*pre, m, n) : at::Tensor();
         const auto options = dy.options().requires_grad(false);

@@ -54,7 +54,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     x [..., k], weight [n, k], bias [n], residual [..., n], all BF16 or all FP16 on one CUDA device, any strides
     (a weight stored as [k, n] is passed as its transpose). activation: "none", "relu", "gelu" (with the error
     function), "gelu_tanh" or "silu". Returns y [..., n], or with save_pre (y, pre), pre = x weight^T + bias before
-    the activation, which linear_backward needs for one. Differentiable with respect to all four tensors.
+    the activation, which linear_backward needs for one. Differentiable with respect to all four tensors, once and in
+    reverse mode: a tangent of the forward mode is refused with RuntimeError.
     Raises ValueError for what does not fit together, RuntimeError for a CUDA failure."""
     out = _torch.linear(x, weight, bias, residual, _activation("linear", activation), bool(save_pre), True)
     if out is None:  # a gradient is wanted
@@ -67,6 +68,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, *, 
                     need_bias: bool = True):
     """The gradients (dx, dweight, dbias) of linear for the gradient dy [..., n] of its output; those not needed are
     None. pre [..., n], linear's second result, is needed with an activation. The gradient of the residual is dy.
-    dy act'(pre) is rounded to the tensors' type once before the products, not before the sum for dbias."""
+    dy act'(pre) is rounded to the tensors' type once before the products, not before the sum for dbias. The results
+    carry no gradients of their own; forward-mode tangents are refused with RuntimeError."""
     return _torch.linear_backward(dy, x, weight, pre, _activation("linear_backward", activation), bool(need_input),
                                   bool(need_weight), bool(need_bias))
