@@ -7,6 +7,8 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
@@ -114,6 +116,23 @@ void refuse_tangents(const char* who, std::initializer_list<const at::Tensor*> a
             throw std::runtime_error(std::string(who) + ": forward-mode differentiation is not supported");
 }
 
+// Whether torch is recording what it dispatches (a tracer, a dispatch mode), or a tensor has no memory of its own to be
+// worked on (a subclass that dispatches, a functional or fake tensor): such a call has to be dispatched itself, since a
+// recorder would keep the results' allocation and never see what is written into them. What must not pass in silence
+// either way is refused: tangents, and the wrapped tensors of torch.func, which may hide some.
+bool is_dispatched(const char* who, std::initializer_list<const at::Tensor*> all) {
+    refuse_tangents(who, all);
+    constexpr c10::DispatchKeySet wrapped({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper});
+    for (const at::Tensor* t : all)
+        if (t && t->key_set().has_any(wrapped))
+            throw std::runtime_error(std::string(who) + ": the transforms of torch.func are not supported");
+    if (c10::impl::dispatch_mode_enabled() || at::tracer::impl::is_dispatch_enabled()) return true;
+    constexpr c10::DispatchKeySet keys({c10::DispatchKey::Python, c10::DispatchKey::Functionalize});
+    for (const at::Tensor* t : all)
+        if (t && t->key_set().has_any(keys)) return true;
+    return false;
+}
+
 PyObject* wrapped(const at::Tensor& t) {
     if (t.defined()) return THPVariable_Wrap(t);
     Py_RETURN_NONE;
@@ -125,15 +144,17 @@ bool expect(Py_ssize_t got, Py_ssize_t wanted, const char* who) {
     return false;
 }
 
-// linear(x, weight, bias, residual, activation, save_pre, differentiable) -> (y, pre or None), or None where a
-// gradient is wanted and `differentiable`: the caller records the call then.
+// linear(x, weight, bias, residual, activation, save_pre, outermost) -> (y, pre or None). A call that a user makes
+// (`outermost`) gives None where a gradient is wanted, and NotImplemented where it has to be dispatched: layers.py
+// makes it again from there.
 PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
     if (!expect(count, 7, "linear")) return nullptr;
     return guarded([&]() -> PyObject* {
         constexpr const char* who = "linear";
         const at::Tensor &x = tensor(args[0], who, "x"), &w = tensor(args[1], who, "weight");
         const at::Tensor *b = tensor_or_none(args[2], who, "bias"), *r = tensor_or_none(args[3], who, "residual");
-        const bool save_pre = args[5] == Py_True;
+        const bool save_pre = args[5] == Py_True, outermost = args[6] == Py_True;
+        if (outermost && is_dispatched(who, {&x, &w, b, r})) Py_RETURN_NOTIMPLEMENTED;
         oztt_linear a{};
         a.format = format_of(x, who);
         same_kind(x, &w, who, "weight");
@@ -153,10 +174,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
         }
         if (r && !(fits && r->size(dim - 1) == n))
             refuse("linear: residual " + text(*r) + " does not match the output of x " + text(x) + " and weight " + text(w));
-        if (args[6] == Py_True) {
-            refuse_tangents(who, {&x, &w, b, r});
-            if (wants_gradient({&x, &w, b, r})) Py_RETURN_NONE;
-        }
+        if (outermost && wants_gradient({&x, &w, b, r})) Py_RETURN_NONE;
         at::NoGradGuard no_grad;
         const at::Tensor x2 = rows_of(x, m, k);
         const at::Tensor r2 = r ? rows_of(*r, m, n) : at::Tensor();
@@ -184,13 +202,15 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
     });
 }
 
-// linear_backward(dy, x, weight, pre, activation, need_input, need_weight, need_bias) -> (dx, dw, db)
+// linear_backward(dy, x, weight, pre, activation, need_input, need_weight, need_bias, outermost) -> (dx, dw, db), or
+// NotImplemented where a user's call has to be dispatched
 PyObject* linear_backward(PyObject*, PyObject* const* args, Py_ssize_t count) {
-    if (!expect(count, 8, "linear_backward")) return nullptr;
+    if (!expect(count, 9, "linear_backward")) return nullptr;
     return guarded([&]() -> PyObject* {
         constexpr const char* who = "linear_backward";
         const at::Tensor &dy = tensor(args[0], who, "dy"), &x = tensor(args[1], who, "x"), &w = tensor(args[2], who, "weight");
         const at::Tensor* pre = tensor_or_none(args[3], who, "pre");
+        if (args[8] == Py_True && is_dispatched(who, {&dy, &x, &w, pre})) Py_RETURN_NOTIMPLEMENTED;
         oztt_linear_grad a{};
         a.format = format_of(dy, who);
         same_kind(dy, &x, who, "x");
@@ -211,7 +231,6 @@ PyObject* linear_backward(PyObject*, PyObject* const* args, Py_ssize_t count) {
         if (a.activation != OZTT_ACT_NONE && !pre) refuse("linear_backward: the activation needs pre");
         if (pre && pre->sizes() != dy.sizes())
             refuse("linear_backward: pre " + text(*pre) + " does not match dy " + text(dy));
-        refuse_tangents(who, {&dy, &x, &w, pre});
         at::NoGradGuard no_grad;
         const at::Tensor x2 = rows_of(x, m, k), dy2 = rows_of(dy, m, n), pre2 = pre ? rows_of(*pre, m, n) : at::Tensor();
         const auto options = dy.options().requires_grad(false);
