@@ -97,9 +97,14 @@ oztt_view view(const at::Tensor& t) {
     const bool matrix = t.dim() == 2;
     return {t.data_ptr(), matrix ? t.stride(0) : 0, t.stride(matrix ? 1 : 0)};
 }
-oztt_view view(const at::Tensor* t) { return t ? view(*t) : oztt_view{nullptr, 0, 0}; }
 
-at::Tensor rows_of(const at::Tensor& t, int64_t rows, int64_t cols) { return t.dim() == 2 ? t : t.reshape({rows, cols}); }
+// A tensor whose memory holds its values: itself, or a copy where torch keeps a negation or a zero for later.
+at::Tensor with_values(const at::Tensor& t) { return t.is_neg() || t._is_zerotensor() ? t.clone() : t; }
+
+at::Tensor rows_of(const at::Tensor& given, int64_t rows, int64_t cols) {
+    const at::Tensor t = with_values(given);
+    return t.dim() == 2 ? t : t.reshape({rows, cols});
+}
 
 bool wants_gradient(std::initializer_list<const at::Tensor*> all) {
     if (!c10::GradMode::is_enabled()) return false;
@@ -176,7 +181,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
             refuse("linear: residual " + text(*r) + " does not match the output of x " + text(x) + " and weight " + text(w));
         if (outermost && wants_gradient({&x, &w, b, r})) Py_RETURN_NONE;
         at::NoGradGuard no_grad;
-        const at::Tensor x2 = rows_of(x, m, k);
+        const at::Tensor x2 = rows_of(x, m, k), w2 = with_values(w), b2 = b ? with_values(*b) : at::Tensor();
         const at::Tensor r2 = r ? rows_of(*r, m, n) : at::Tensor();
         at::Tensor y = at::empty({m, n}, x.options().requires_grad(false)), pre;
         if (save_pre) pre = at::empty_like(y);
@@ -184,8 +189,8 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
         a.n = (uint64_t)n;
         a.k = (uint64_t)k;
         a.x = view(x2);
-        a.w = view(w);
-        a.bias = view(b);
+        a.w = view(w2);
+        if (b) a.bias = view(b2);
         if (r) a.residual = view(r2);
         a.y = view(y);
         if (save_pre) a.pre = view(pre);
@@ -232,7 +237,8 @@ PyObject* linear_backward(PyObject*, PyObject* const* args, Py_ssize_t count) {
         if (pre && pre->sizes() != dy.sizes())
             refuse("linear_backward: pre " + text(*pre) + " does not match dy " + text(dy));
         at::NoGradGuard no_grad;
-        const at::Tensor x2 = rows_of(x, m, k), dy2 = rows_of(dy, m, n), pre2 = pre ? rows_of(*pre, m, n) : at::Tensor();
+        const at::Tensor x2 = rows_of(x, m, k), w2 = with_values(w), dy2 = rows_of(dy, m, n);
+        const at::Tensor pre2 = pre ? rows_of(*pre, m, n) : at::Tensor();
         const auto options = dy.options().requires_grad(false);
         at::Tensor dx, dw, db;
         if (args[5] == Py_True) dx = at::empty({m, k}, options);
@@ -243,7 +249,7 @@ PyObject* linear_backward(PyObject*, PyObject* const* args, Py_ssize_t count) {
         a.k = (uint64_t)k;
         a.dy = view(dy2);
         a.x = view(x2);
-        a.w = view(w);
+        a.w = view(w2);
         if (pre) a.pre = view(pre2);
         if (dx.defined()) a.dx = view(dx);
         if (dw.defined()) a.dw = view(dw);
