@@ -280,10 +280,32 @@ PyObject** items(PyObject* o, Py_ssize_t n, const char* what) {
     return PySequence_Fast_ITEMS(o);
 }
 
+// The record of the moments (m, v, m_exp, v_exp) of `blocks` blocks, the exponents None with 32 bits. Their addresses
+// are asked for in every call: a copy of an optimiser has other buffers than the original.
+oztt_adamw_moments moments_of(PyObject* four, uint64_t blocks, int device) {
+    if (!PyTuple_Check(four) || PyTuple_GET_SIZE(four) != 4) throw std::runtime_error("AdamW: the moments are four buffers");
+    const auto buffer = [&](int i, bool wide, uint64_t count) -> void* {
+        const at::Tensor* t = tensor_or_none(PyTuple_GET_ITEM(four, i), "AdamW", "a buffer of the moments");
+        if (!t || !t->is_cuda() || t->get_device() != device || t->scalar_type() != (wide ? at::kFloat : at::kByte) ||
+            (uint64_t)t->numel() != count || !t->is_contiguous())
+            refuse("AdamW: a buffer of the moments is not what it was made as");
+        return t->data_ptr();
+    };
+    oztt_adamw_moments m{};
+    m.bits = PyTuple_GET_ITEM(four, 2) == Py_None ? 32 : 8;
+    m.m = buffer(0, m.bits == 32, blocks * OZTT_ADAMW_BLOCK);
+    m.v = buffer(1, m.bits == 32, blocks * OZTT_ADAMW_BLOCK);
+    if (m.bits == 8) {
+        m.m_exp = static_cast<uint8_t*>(buffer(2, false, blocks));
+        m.v_exp = static_cast<uint8_t*>(buffer(3, false, blocks));
+    }
+    return m;
+}
+
 // adamw_step(table, params, masters, grads, grad_scale, moments, hyper, device): table a writable buffer of
 // oztt_adamw_tensor, one for each parameter, with the count and type that it was made for; the addresses, which a
-// program may change between steps, are filled in here. masters and grads may hold None; moments and hyper are bytes
-// of oztt_adamw_moments and oztt_adamw_hyper (with grad_scale filled in here).
+// program may change between steps, are filled in here. masters and grads may hold None; moments are the four
+// buffers, hyper the bytes of oztt_adamw_hyper (with grad_scale filled in here).
 PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
     if (!expect(count, 8, "adamw_step")) return nullptr;
     Py_buffer table;
@@ -294,6 +316,9 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
         PyObject **params = items(args[1], n, "params"), **masters = items(args[2], n, "masters"),
                  **grads = items(args[3], n, "grads");
         const int device = (int)PyLong_AsLong(args[7]);
+        uint64_t blocks = 0;
+        for (Py_ssize_t i = 0; i < n; ++i) blocks += (t[i].count + OZTT_ADAMW_BLOCK - 1) / OZTT_ADAMW_BLOCK;
+        const oztt_adamw_moments moments = moments_of(args[5], blocks, device);
         for (Py_ssize_t i = 0; i < n; ++i) {
             const auto address = [&](const at::Tensor& x, const char* what) -> void* {
                 const auto which = [&] { return std::string("AdamW: ") + what + " " + std::to_string(i); };
@@ -315,11 +340,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
             if (w && w->scalar_type() != at::kFloat) refuse("AdamW: master " + std::to_string(i) + " must be FP32");
             t[i].master = w ? static_cast<float*>(address(*w, "master")) : nullptr;
         }
-        oztt_adamw_moments moments;
         oztt_adamw_hyper hyper;
-        if (PyBytes_GET_SIZE(args[5]) != sizeof moments || PyBytes_GET_SIZE(args[6]) != sizeof hyper)
-            throw std::runtime_error("adamw_step: records of another size");
-        std::memcpy(&moments, PyBytes_AS_STRING(args[5]), sizeof moments);
+        if (PyBytes_GET_SIZE(args[6]) != sizeof hyper) throw std::runtime_error("adamw_step: a record of another size");
         std::memcpy(&hyper, PyBytes_AS_STRING(args[6]), sizeof hyper);
         if (const at::Tensor* s = tensor_or_none(args[4], "AdamW", "grad_scale")) {
             if (s->scalar_type() != at::kFloat || !s->is_cuda() || s->get_device() != device || s->numel() != 1)
@@ -338,11 +360,9 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
 PyObject* adamw_values(PyObject*, PyObject* const* args, Py_ssize_t count) {
     if (!expect(count, 3, "adamw_values")) return nullptr;
     return guarded([&]() -> PyObject* {
-        oztt_adamw_moments moments;
-        if (PyBytes_GET_SIZE(args[0]) != sizeof moments) throw std::runtime_error("adamw_values: a record of another size");
-        std::memcpy(&moments, PyBytes_AS_STRING(args[0]), sizeof moments);
         const int64_t blocks = PyLong_AsLongLong(args[1]);
         const int device = (int)PyLong_AsLong(args[2]);
+        const oztt_adamw_moments moments = moments_of(args[0], (uint64_t)blocks, device);
         const auto options = at::TensorOptions(at::kBFloat16).device(at::kCUDA, (c10::DeviceIndex)device);
         const at::Tensor m = at::empty({blocks * OZTT_ADAMW_BLOCK}, options), v = at::empty_like(m);
         void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();

@@ -15,10 +15,9 @@ __all__ = ["AdamW"]
 BLOCK = 256  # OZTT_ADAMW_BLOCK: elements of the moments that share an exponent
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # OZTT_TYPE_*
 
-# oztt_adamw_tensor, oztt_adamw_moments and oztt_adamw_hyper
+# oztt_adamw_tensor and oztt_adamw_hyper
 _TENSOR = np.dtype([("param", np.uint64), ("grad", np.uint64), ("master", np.uint64), ("count", np.uint64),
                     ("param_type", np.int32), ("grad_type", np.int32)])
-_MOMENTS = struct.Struct("=i4x4Q")
 _HYPER = struct.Struct("=5dQQI4x")
 
 _torch = _binding()  # csrc/torch_binding.cpp: the tensors' checks and addresses, the current stream
@@ -85,8 +84,6 @@ class AdamW:
         self._table["count"] = self._counts
         self._table["param_type"] = [_TYPES[p.dtype] for p in params]
         self._grown = [p for p in params if p.requires_grad]
-        exps = (self._m_exp.data_ptr(), self._v_exp.data_ptr()) if state_bits == 8 else (0, 0)
-        self._record = _MOMENTS.pack(state_bits, self._m.data_ptr(), self._v.data_ptr(), *exps)
 
     def step(self, grads=None, *, grad_scale: torch.Tensor | None = None, lr: float | None = None,
              seed: int | None = None) -> None:
@@ -103,8 +100,8 @@ class AdamW:
             seed = self.seed + 0x632BE5AB * t
         hyper = _HYPER.pack(self.lr if lr is None else lr, *self.betas, self.eps, self.weight_decay, t,
                             0, seed & 0xFFFFFFFF)
-        _torch.adamw_step(self._table, self.params, self.masters, grads, grad_scale, self._record, hyper,
-                          self.device.index)
+        _torch.adamw_step(self._table, self.params, self.masters, grads, grad_scale,
+                          (self._m, self._v, self._m_exp, self._v_exp), hyper, self.device.index)
         self.t = t
         if self._grown:  # saved for a backward pass that has not run, they are no longer what was saved
             torch.autograd.graph.increment_version(self._grown)
@@ -120,7 +117,7 @@ class AdamW:
         BF16 tensors with 8, which hold the values of the codes exactly."""
         if self.state_bits == 32:
             return self._m, self._v
-        return _torch.adamw_values(self._record, self.blocks, self.device.index)
+        return _torch.adamw_values((self._m, self._v, self._m_exp, self._v_exp), self.blocks, self.device.index)
 
     def state_dict(self) -> dict:
         """What load_state_dict needs to go on from here: the number of steps, the moments as they are kept, and the
