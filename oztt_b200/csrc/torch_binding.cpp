@@ -273,6 +273,25 @@ int32_t type_of(const at::Tensor& t) {
     }
 }
 
+// Whether a tensor is its memory: not one that dispatches elsewhere (a subclass, a wrapped, functional or fake tensor),
+// nor one that keeps a negation or a zero for later.
+bool is_memory(const at::Tensor& t) {
+    constexpr c10::DispatchKeySet keys({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
+                                        c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize,
+                                        c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor});
+    return !t.key_set().has_any(keys);
+}
+
+// A tracer, or a mode that records programs or computes shapes alone, sees nothing of what is written here.
+void refuse_recorders(const char* who) {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    bool some = at::tracer::impl::is_dispatch_enabled();
+    for (const auto key : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+        some = some || TorchDispatchModeTLS::get_mode(key).has_value();
+    if (some) throw std::runtime_error(std::string(who) + " cannot be traced or recorded");
+}
+
 // The items of a list or tuple of n.
 PyObject** items(PyObject* o, Py_ssize_t n, const char* what) {
     if (!PyList_Check(o) && !PyTuple_Check(o)) refuse(std::string("AdamW: ") + what + " must be a list or a tuple");
@@ -311,6 +330,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
     Py_buffer table;
     if (PyObject_GetBuffer(args[0], &table, PyBUF_WRITABLE) != 0) return nullptr;
     PyObject* result = guarded([&]() -> PyObject* {
+        refuse_recorders("AdamW.step");
         auto* t = static_cast<oztt_adamw_tensor*>(table.buf);
         const Py_ssize_t n = table.len / (Py_ssize_t)sizeof(oztt_adamw_tensor);
         PyObject **params = items(args[1], n, "params"), **masters = items(args[2], n, "masters"),
@@ -325,6 +345,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
                 if (!x.is_cuda() || x.get_device() != device) refuse(which() + " must be on the parameters' device");
                 if ((uint64_t)x.numel() != t[i].count) refuse(which() + " has not its parameter's size");
                 if (!x.is_contiguous()) refuse(which() + " must be contiguous");
+                if (!is_memory(x)) refuse(which() + " has no memory of its own values");
                 return x.data_ptr();
             };
             t[i].grad = nullptr;
@@ -344,7 +365,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
         if (PyBytes_GET_SIZE(args[6]) != sizeof hyper) throw std::runtime_error("adamw_step: a record of another size");
         std::memcpy(&hyper, PyBytes_AS_STRING(args[6]), sizeof hyper);
         if (const at::Tensor* s = tensor_or_none(args[4], "AdamW", "grad_scale")) {
-            if (s->scalar_type() != at::kFloat || !s->is_cuda() || s->get_device() != device || s->numel() != 1)
+            if (s->scalar_type() != at::kFloat || !s->is_cuda() || s->get_device() != device || s->numel() != 1 || !is_memory(*s))
                 refuse("AdamW: grad_scale must be one FP32 number on the parameters' device");
             hyper.grad_scale = s->const_data_ptr<float>();
         }
@@ -360,6 +381,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
 PyObject* adamw_values(PyObject*, PyObject* const* args, Py_ssize_t count) {
     if (!expect(count, 3, "adamw_values")) return nullptr;
     return guarded([&]() -> PyObject* {
+        refuse_recorders("AdamW.moments");
         const int64_t blocks = PyLong_AsLongLong(args[1]);
         const int device = (int)PyLong_AsLong(args[2]);
         const oztt_adamw_moments moments = moments_of(args[0], (uint64_t)blocks, device);
@@ -374,11 +396,18 @@ PyObject* adamw_values(PyObject*, PyObject* const* args, Py_ssize_t count) {
     });
 }
 
+// has_memory(tensor) -> bool
+PyObject* has_memory(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    if (!expect(count, 1, "has_memory")) return nullptr;
+    return guarded([&]() -> PyObject* { return PyBool_FromLong(is_memory(tensor(args[0], "AdamW", "a parameter"))); });
+}
+
 PyMethodDef methods[] = {
     {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear)), METH_FASTCALL, nullptr},
     {"linear_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear_backward)), METH_FASTCALL, nullptr},
     {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(adamw_step)), METH_FASTCALL, nullptr},
     {"adamw_values", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(adamw_values)), METH_FASTCALL, nullptr},
+    {"has_memory", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(has_memory)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -54,11 +54,12 @@ class AdamW:
             raise ValueError("AdamW: masters must be as many as params")
         spans = []
         for i, (p, w) in enumerate(zip(params, masters)):
-            if p.dtype not in _TYPES or p.device != device or not p.is_contiguous():
+            if p.dtype not in _TYPES or p.device != device or not p.is_contiguous() or not _torch.has_memory(p):
                 raise ValueError(f"AdamW: parameter {i} must be a contiguous BF16, FP16 or FP32 tensor on {device}")
             spans.append((p.data_ptr(), p.numel() * p.element_size()))
             if w is not None:
-                if w.dtype != torch.float32 or w.device != device or not w.is_contiguous() or w.shape != p.shape:
+                if (w.dtype != torch.float32 or w.device != device or not w.is_contiguous() or w.shape != p.shape
+                        or not _torch.has_memory(w)):
                     raise ValueError(f"AdamW: master {i} must be a contiguous FP32 tensor like its parameter")
                 spans.append((w.data_ptr(), w.numel() * 4))
         end = 0
