@@ -122,6 +122,16 @@ __device__ __forceinline__ f32x2 activate2(f32x2 z) {
     }
     return z;
 }
+// Both values within [-64, 64], NaN kept.
+__device__ __forceinline__ f32x2 within_64(f32x2 x) {
+    float a, b;
+    unpk2(x, a, b);
+    asm("min.NaN.f32 %0, %0, 0f42800000;" : "+f"(a));
+    asm("min.NaN.f32 %0, %0, 0f42800000;" : "+f"(b));
+    asm("max.NaN.f32 %0, %0, 0fC2800000;" : "+f"(a));
+    asm("max.NaN.f32 %0, %0, 0fC2800000;" : "+f"(b));
+    return pk2(a, b);
+}
 // dz of a pair: dy times the activation's derivative at z.
 template <int ACT>
 __device__ __forceinline__ f32x2 through_slope2(f32x2 dy, f32x2 z) {
@@ -142,6 +152,7 @@ __device__ __forceinline__ f32x2 through_slope2(f32x2 dy, f32x2 z) {
             zu = z;
         } else {
             constexpr float c = -2.0f * kTanhScale * kLog2e;
+            z = within_64(z);  // the slope is 0 or 1 long before; the cube below would leave the range from 1.2e13 on
             const f32x2 zz = times2(z, z);
             s = logistic2(times2(z, fma2(splat2(c * kTanhCube), zz, splat2(c))));
             zu = times2(z, fma2(splat2(6.0f * kTanhScale * kTanhCube), zz, splat2(2.0f * kTanhScale)));
