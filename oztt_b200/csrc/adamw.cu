@@ -71,18 +71,6 @@ struct Hyper {
     const float* grad_scale;
 };
 
-// ---- pairs of 32-bit values, without flushing: first element in the low half ---------------------
-__device__ __forceinline__ f32x2 plus2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 fused2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
 // Eight neighbouring elements as they lie in memory: 16-bit ones in the first four words.
 template <bool WIDE>
 struct Words {

@@ -57,12 +57,9 @@ struct Epilogue {
 
 // ---- activations in 32 bits ----------------------------------------------------------------------
 // On pairs of values (one instruction of the packed FP32 pipe each), with the two special functions 2^x and 1/x by
-// the hardware's approximations (2^-22): a pass over dz issues 10 instructions an element so, 26 with scalar ones.
-__device__ __forceinline__ f32x2 times2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
+// the hardware's approximations (2^-22): a pass over dz issues 10 instructions an element so, 26 with scalar ones. Only
+// those two flush: a factor 2^x below 2^-126 is zero, so results below |z| 2^-126 in size may be too. Sums, biases,
+// residuals and products keep subnormal values, as the tensor cores do.
 __device__ __forceinline__ f32x2 exp2_2(f32x2 x) {
     float a, b;
     unpk2(x, a, b);
@@ -82,7 +79,7 @@ constexpr float kTanhScale = 0.7978845608028654f;  // sqrt(2/pi)
 constexpr float kTanhCube = 0.044715f;
 
 // 1 / (1 + 2^x): the logistic function of -x ln 2
-__device__ __forceinline__ f32x2 logistic2(f32x2 x) { return reciprocal2(add2(splat2(1.0f), exp2_2(x))); }
+__device__ __forceinline__ f32x2 logistic2(f32x2 x) { return reciprocal2(plus2(splat2(1.0f), exp2_2(x))); }
 
 // The normal distribution's cumulative function, and e = exp(-z^2 / 2) on the way: the rational approximation
 // 7.1.26 of Abramowitz and Stegun's Handbook of Mathematical Functions (erfc x = t (a1 + t (a2 + ...)) exp(-x^2),
@@ -90,11 +87,11 @@ __device__ __forceinline__ f32x2 logistic2(f32x2 x) { return reciprocal2(add2(sp
 // for the lower tail, no cancellation.
 __device__ __forceinline__ f32x2 normal_cdf2(f32x2 z, f32x2& e) {
     const f32x2 size = z & 0x7FFFFFFF7FFFFFFFull;
-    const f32x2 t = reciprocal2(fma2(splat2(0.3275911f * 0.70710678118654752f), size, splat2(1.0f)));
-    f32x2 q = fma2(splat2(0.5f * 1.061405429f), t, splat2(0.5f * -1.453152027f));
-    q = fma2(q, t, splat2(0.5f * 1.421413741f));
-    q = fma2(q, t, splat2(0.5f * -0.284496736f));
-    q = fma2(q, t, splat2(0.5f * 0.254829592f));
+    const f32x2 t = reciprocal2(fused2(splat2(0.3275911f * 0.70710678118654752f), size, splat2(1.0f)));
+    f32x2 q = fused2(splat2(0.5f * 1.061405429f), t, splat2(0.5f * -1.453152027f));
+    q = fused2(q, t, splat2(0.5f * 1.421413741f));
+    q = fused2(q, t, splat2(0.5f * -0.284496736f));
+    q = fused2(q, t, splat2(0.5f * 0.254829592f));
     e = exp2_2(times2(times2(z, splat2(-0.5f * kLog2e)), z));
     float tail0, tail1, z0, z1;
     unpk2(times2(times2(q, t), e), tail0, tail1);
@@ -116,7 +113,7 @@ __device__ __forceinline__ f32x2 activate2(f32x2 z) {
         return times2(z, normal_cdf2(z, e));
     } else if constexpr (ACT == OZTT_ACT_GELU_TANH) {
         constexpr float c = -2.0f * kTanhScale * kLog2e;
-        return times2(z, logistic2(times2(z, fma2(splat2(c * kTanhCube), times2(z, z), splat2(c)))));
+        return times2(z, logistic2(times2(z, fused2(splat2(c * kTanhCube), times2(z, z), splat2(c)))));
     } else if constexpr (ACT == OZTT_ACT_SILU) {
         return times2(z, logistic2(times2(z, splat2(-kLog2e))));
     }
@@ -143,7 +140,7 @@ __device__ __forceinline__ f32x2 through_slope2(f32x2 dy, f32x2 z) {
     } else if constexpr (ACT == OZTT_ACT_GELU) {
         f32x2 e;
         const f32x2 c = normal_cdf2(z, e);
-        return times2(dy, fma2(times2(z, splat2(0.3989422804014327f)), e, c));
+        return times2(dy, fused2(times2(z, splat2(0.3989422804014327f)), e, c));
     } else if constexpr (ACT == OZTT_ACT_GELU_TANH || ACT == OZTT_ACT_SILU) {
         // z s(u) with s the logistic function: s + z u' s (1 - s) = s (1 + z u' (1 - s))
         f32x2 s, zu;
@@ -154,10 +151,10 @@ __device__ __forceinline__ f32x2 through_slope2(f32x2 dy, f32x2 z) {
             constexpr float c = -2.0f * kTanhScale * kLog2e;
             z = within_64(z);  // the slope is 0 or 1 long before; the cube below would leave the range from 1.2e13 on
             const f32x2 zz = times2(z, z);
-            s = logistic2(times2(z, fma2(splat2(c * kTanhCube), zz, splat2(c))));
-            zu = times2(z, fma2(splat2(6.0f * kTanhScale * kTanhCube), zz, splat2(2.0f * kTanhScale)));
+            s = logistic2(times2(z, fused2(splat2(c * kTanhCube), zz, splat2(c))));
+            zu = times2(z, fused2(splat2(6.0f * kTanhScale * kTanhCube), zz, splat2(2.0f * kTanhScale)));
         }
-        return times2(times2(dy, s), fma2(zu, sub2(splat2(1.0f), s), splat2(1.0f)));
+        return times2(times2(dy, s), fused2(zu, sub2(splat2(1.0f), s), splat2(1.0f)));
     }
     return dy;
 }
@@ -324,7 +321,7 @@ __device__ __forceinline__ void finish_vector(uint16_t* out, uint16_t* pre, bool
     activate_all<N>(z, act);
     if (has_res) {
 #pragma unroll
-        for (int q = 0; q < N; ++q) z[q] = add2(z[q], unpack<HALF>(r[q]));
+        for (int q = 0; q < N; ++q) z[q] = plus2(z[q], unpack<HALF>(r[q]));
     }
 #pragma unroll
     for (int q = 0; q < N; ++q) w[q] = pack<HALF>(z[q]);
@@ -368,7 +365,7 @@ __device__ __forceinline__ void finish_scattered(const Scattered& at, uint32_t c
     if (at.res) {
 #pragma unroll
         for (int q = 0; q < (N + 1) / 2; ++q)
-            z[q] = add2(z[q], pk2(to_f32<HALF>(r[2 * q]), 2 * q + 1 < N ? to_f32<HALF>(r[2 * q + 1 < N ? 2 * q + 1 : 0]) : 0.0f));
+            z[q] = plus2(z[q], pk2(to_f32<HALF>(r[2 * q]), 2 * q + 1 < N ? to_f32<HALF>(r[2 * q + 1 < N ? 2 * q + 1 : 0]) : 0.0f));
     }
     store(at.out, at.out_step);
 }
@@ -784,7 +781,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             const ulonglong2 x = b[q];
-                            z[2 * q] = add2(z[2 * q], x.x), z[2 * q + 1] = add2(z[2 * q + 1], x.y);
+                            z[2 * q] = plus2(z[2 * q], x.x), z[2 * q + 1] = plus2(z[2 * q + 1], x.y);
                         }
                     }
                     if (!mine) continue;
@@ -840,7 +837,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     __syncwarp();
                     const ulonglong2* p = reinterpret_cast<const ulonglong2*>(patch + prow * PATCH_LD + pcol);
                     const ulonglong2 x = p[0], y = p[1];
-                    f32x2 z[4] = {add2(x.x, bias[0]), add2(x.y, bias[1]), add2(y.x, bias[2]), add2(y.y, bias[3])};
+                    f32x2 z[4] = {plus2(x.x, bias[0]), plus2(x.y, bias[1]), plus2(y.x, bias[2]), plus2(y.y, bias[3])};
                     if (mine) finish_vector<HALF, 4>(out, has_pre ? pre : nullptr, has_res, e.act, z, r);
                     out += PATCH_ROWS * e.out.rs;
                     pre += PATCH_ROWS * e.pre.rs;
@@ -924,7 +921,7 @@ __global__ void __launch_bounds__(256)
                     for (int c = 0; c < FEW_COLS; ++c) {
                         const f32x2 v = unpack<HALF>(w[a][c][h]);
 #pragma unroll
-                        for (int m = 0; m < M; ++m) acc[m][c] = fma2(v, unpack<HALF>(x[a][m][h]), acc[m][c]);
+                        for (int m = 0; m < M; ++m) acc[m][c] = fused2(v, unpack<HALF>(x[a][m][h]), acc[m][c]);
                     }
         } else {
             uint16_t w[AHEAD][FEW_COLS], x[AHEAD][M];
@@ -942,7 +939,7 @@ __global__ void __launch_bounds__(256)
                 for (int c = 0; c < FEW_COLS; ++c)
 #pragma unroll
                     for (int m = 0; m < M; ++m)
-                        acc[m][c] = fma2(pk2(to_f32<HALF>(w[a][c]), to_f32<HALF>(w[a + 1][c])),
+                        acc[m][c] = fused2(pk2(to_f32<HALF>(w[a][c]), to_f32<HALF>(w[a + 1][c])),
                                          pk2(to_f32<HALF>(x[a][m]), to_f32<HALF>(x[a + 1][m])), acc[m][c]);
         }
     }
@@ -1009,7 +1006,7 @@ __global__ void __launch_bounds__(256)
         for (uint32_t t = 0; t < T; ++t) {
             const f32x2 a = splat2(factors[r0 + r][t]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) sum[c] = fma2(a, x[t][c], sum[c]);
+            for (int c = 0; c < 4; ++c) sum[c] = fused2(a, x[t][c], sum[c]);
         }
         uint32_t w[4];
 #pragma unroll
@@ -1152,7 +1149,7 @@ __global__ void __launch_bounds__(256, !VEC ? 3 : ACT == OZTT_ACT_NONE ? 8 : 4)
                 for (int q = 0; q < 4; ++q) {
                     f32x2 v = unpack<HALF>(g[a][q]);
                     if (ACT != OZTT_ACT_NONE) v = through_slope2<ACT>(v, unpack<HALF>(s[a][q]));
-                    sum[q] = add2(sum[q], v);
+                    sum[q] = plus2(sum[q], v);
                     w[q] = pack<HALF>(v);
                 }
                 if (!dz) continue;
