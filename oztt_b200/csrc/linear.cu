@@ -81,17 +81,19 @@ constexpr float kTanhCube = 0.044715f;
 // 1 / (1 + 2^x): the logistic function of -x ln 2
 __device__ __forceinline__ f32x2 logistic2(f32x2 x) { return reciprocal2(plus2(splat2(1.0f), exp2_2(x))); }
 
-// The normal distribution's cumulative function, and e = exp(-z^2 / 2) on the way: the rational approximation
-// 7.1.26 of Abramowitz and Stegun's Handbook of Mathematical Functions (erfc x = t (a1 + t (a2 + ...)) exp(-x^2),
-// t = 1 / (1 + p x), off by at most 1.5e-7, which the 16-bit results do not show). It has no branch and, formed
-// for the lower tail, no cancellation.
+// The normal distribution's cumulative function, and e = exp(-z^2 / 2) on the way. In the lower tail it is
+// e erfcx(|z| / sqrt 2) / 2, and that factor, smooth and between 1/2 and 0, is t (a1 + t (a2 + ... + t a6)) with
+// t = 1 / (1 + 0.29 |z|): coefficients fitted for the least of the largest errors, by linear programming over a grid of
+// [0, 13.6], within 2^-13.8 of itself everywhere and 8.1e-8 absolutely. So the tail is right relative to its own size as
+// far as BF16 reaches, and the upper half to 2.5e-7 in 32-bit arithmetic. No branch, and no cancellation.
 __device__ __forceinline__ f32x2 normal_cdf2(f32x2 z, f32x2& e) {
     const f32x2 size = z & 0x7FFFFFFF7FFFFFFFull;
-    const f32x2 t = reciprocal2(fused2(splat2(0.3275911f * 0.70710678118654752f), size, splat2(1.0f)));
-    f32x2 q = fused2(splat2(0.5f * 1.061405429f), t, splat2(0.5f * -1.453152027f));
-    q = fused2(q, t, splat2(0.5f * 1.421413741f));
-    q = fused2(q, t, splat2(0.5f * -0.284496736f));
-    q = fused2(q, t, splat2(0.5f * 0.254829592f));
+    const f32x2 t = reciprocal2(fused2(splat2(0.29f), size, splat2(1.0f)));
+    f32x2 q = fused2(splat2(-0.0882913856f), t, splat2(0.283034694f));
+    q = fused2(q, t, splat2(-0.0906950769f));
+    q = fused2(q, t, splat2(0.177939345f));
+    q = fused2(q, t, splat2(0.101187212f));
+    q = fused2(q, t, splat2(0.116825293f));
     e = exp2_2(times2(times2(z, splat2(-0.5f * kLog2e)), z));
     float tail0, tail1, z0, z1;
     unpk2(times2(times2(q, t), e), tail0, tail1);
