@@ -292,12 +292,19 @@ void refuse_recorders(const char* who) {
     if (some) throw std::runtime_error(std::string(who) + " cannot be traced or recorded");
 }
 
-// The items of a list or tuple of n.
-PyObject** items(PyObject* o, Py_ssize_t n, const char* what) {
-    if (!PyList_Check(o) && !PyTuple_Check(o)) refuse(std::string("AdamW: ") + what + " must be a list or a tuple");
-    if (PySequence_Fast_GET_SIZE(o) != n) refuse(std::string("AdamW: ") + what + " must be as many as params");
-    return PySequence_Fast_ITEMS(o);
-}
+// The items of a list or tuple of n, held for the call: another thread may change the list while the lock is released.
+struct Items {
+    PyObject* held;
+    Items(PyObject* o, Py_ssize_t n, const char* what) {
+        if (!PyList_Check(o) && !PyTuple_Check(o)) refuse(std::string("AdamW: ") + what + " must be a list or a tuple");
+        if (PySequence_Fast_GET_SIZE(o) != n) refuse(std::string("AdamW: ") + what + " must be as many as params");
+        held = PySequence_Tuple(o);
+        if (!held) throw std::bad_alloc();
+    }
+    ~Items() { Py_DECREF(held); }
+    Items(const Items&) = delete;
+    PyObject* operator[](Py_ssize_t i) const { return PyTuple_GET_ITEM(held, i); }
+};
 
 // The record of the moments (m, v, m_exp, v_exp) of `blocks` blocks, the exponents None with 32 bits. Their addresses
 // are asked for in every call: a copy of an optimiser has other buffers than the original.
@@ -333,8 +340,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
         refuse_recorders("AdamW.step");
         auto* t = static_cast<oztt_adamw_tensor*>(table.buf);
         const Py_ssize_t n = table.len / (Py_ssize_t)sizeof(oztt_adamw_tensor);
-        PyObject **params = items(args[1], n, "params"), **masters = items(args[2], n, "masters"),
-                 **grads = items(args[3], n, "grads");
+        const Items params(args[1], n, "params"), masters(args[2], n, "masters"), grads(args[3], n, "grads");
         const int device = (int)PyLong_AsLong(args[7]);
         uint64_t blocks = 0;
         for (Py_ssize_t i = 0; i < n; ++i) blocks += (t[i].count + OZTT_ADAMW_BLOCK - 1) / OZTT_ADAMW_BLOCK;
@@ -371,6 +377,18 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
         }
         void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
         call([&](char* err, size_t len) { return oztt_adamw_step(device, t, (uint64_t)n, &moments, &hyper, stream, err, len); });
+        // what was saved for a backward pass that has not run is no longer what it was
+        const auto written = [](PyObject* o) {
+            if (o == Py_None) return;
+            const at::Tensor& x = THPVariable_Unpack(o);
+            if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+        };
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            if (grads[i] == Py_None) continue;
+            written(params[i]);
+            written(masters[i]);
+        }
+        for (Py_ssize_t i = 0; i < 4; ++i) written(PyTuple_GET_ITEM(args[5], i));
         Py_RETURN_NONE;
     });
     PyBuffer_Release(&table);

@@ -84,7 +84,6 @@ class AdamW:
         self._table = np.zeros(len(params), _TENSOR)
         self._table["count"] = self._counts
         self._table["param_type"] = [_TYPES[p.dtype] for p in params]
-        self._grown = [p for p in params if p.requires_grad]
 
     def step(self, grads=None, *, grad_scale: torch.Tensor | None = None, lr: float | None = None,
              seed: int | None = None) -> None:
@@ -93,7 +92,7 @@ class AdamW:
         .grad. grad_scale: one FP32 number on the device that every gradient is multiplied by (a clipping
         coefficient). lr: this step's learning rate. seed: of this step's rounding, by default from the optimiser's
         seed and the step's number. The step's number and rates are numbers of the launch: a CUDA graph of it
-        repeats the same step."""
+        repeats the same step. The versions of what is stepped are raised, as by torch's own operations in place."""
         if grads is None:
             grads = [p.grad for p in self.params]
         t = self.t + 1
@@ -104,8 +103,6 @@ class AdamW:
         _torch.adamw_step(self._table, self.params, self.masters, grads, grad_scale,
                           (self._m, self._v, self._m_exp, self._v_exp), hyper, self.device.index)
         self.t = t
-        if self._grown:  # saved for a backward pass that has not run, they are no longer what was saved
-            torch.autograd.graph.increment_version(self._grown)
 
     # The moments as they are kept: FP32, or bytes with the blocks' exponents.
     m = property(lambda self: self._m)
