@@ -7,6 +7,12 @@
 
 namespace oztt {
 
+// The word that a bounded wait of a layer product writes when it gives up: host memory that every device reaches. These
+// calls do not wait for their kernels, so the next of them, or the optimiser's call that would use what they computed,
+// looks at it and throws (linear.cu).
+int* error_word();
+void check_earlier_calls();
+
 // Makes `device` current for one call.
 struct DeviceScope {
     int before = 0;

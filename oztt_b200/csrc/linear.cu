@@ -27,6 +27,31 @@
 #include "tensor_core.cuh"
 
 namespace oztt {
+
+// Both of launch.cuh.
+static std::atomic<int*> known_word{nullptr};
+int* error_word() {
+    static std::once_flag once;
+    std::call_once(once, [] {
+        int* word = nullptr;
+        if (cudaHostAlloc(&word, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
+            *word = 0;
+            known_word = word;
+        } else {
+            cudaGetLastError();
+        }
+    });
+    if (!known_word) throw Error(OZTT_ERUNTIME, "linear: no pinned host memory for the error word");
+    return known_word;
+}
+void check_earlier_calls() {
+    int* word = known_word;
+    if (!word) return;  // no product has run
+    if (const int code = __atomic_exchange_n(word, 0, __ATOMIC_RELAXED))
+        throw Error(OZTT_ERUNTIME, "linear: a kernel of an earlier call gave up waiting (code " + std::to_string(code) +
+                                       "); that call's outputs are not valid");
+}
+
 namespace layer {
 
 using namespace gemm;
@@ -1219,29 +1244,6 @@ __global__ void __launch_bounds__(256) db_kernel(const float* partial, uint64_t 
 
 // ---- host side -----------------------------------------------------------------------------------
 
-// The word that a kernel's bounded wait writes when it gives up: host memory that every device reaches, looked
-// at by the next call, since these calls do not wait for their kernels.
-static int* error_word() {
-    static int* word = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        if (cudaHostAlloc(&word, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess)
-            *word = 0;
-        else
-            word = nullptr, cudaGetLastError();
-    });
-    if (!word) throw Error(OZTT_ERUNTIME, "linear: no pinned host memory for the error word");
-    return word;
-}
-static void check_earlier_calls() {
-    volatile int* w = error_word();
-    if (const int code = *w) {
-        *w = 0;
-        throw Error(OZTT_ERUNTIME, "linear: a kernel of an earlier call gave up waiting (code " + std::to_string(code) +
-                                       "); that call's outputs are not valid");
-    }
-}
-
 // Operand of a product: rows x red elements, element (r, t) at p[r * rs + t * ks].
 struct Operand {
     const void* p;
@@ -1720,5 +1722,5 @@ extern "C" int oztt_linear_backward(int device_id, const oztt_linear_grad* args,
 
 // Puts a wait's error code where a kernel would have put it, for the test of how the next call reports it.
 extern "C" int oztt_test_linear_error(int32_t code, char* err, size_t errlen) {
-    return oztt::guarded(err, errlen, [&] { *oztt::layer::error_word() = code; });
+    return oztt::guarded(err, errlen, [&] { *oztt::error_word() = code; });
 }
