@@ -440,8 +440,7 @@ int oztt_get_option(int32_t option, int32_t* value);
  * Any strides are taken; operands whose rows start on 16 bytes (and outputs whose rows start on 8) are read and
  * written as they lie, others cost a copy of the operand. Outputs must not overlap operands, except y the
  * residual it is computed from. A kernel that gives up a wait is reported by the next call, an optimiser's included
- * (OZTT_ERUNTIME, with nothing done). Make the process's first call before any stream capture (it allocates the word
- * that such a kernel writes). */
+ * (OZTT_ERUNTIME, with nothing done). */
 enum { OZTT_ACT_NONE = 0, OZTT_ACT_RELU = 1, OZTT_ACT_GELU = 2, OZTT_ACT_GELU_TANH = 3, OZTT_ACT_SILU = 4 };
 
 /* A matrix (or, with row_stride unused, a vector) by its strides in elements; data may be NULL where the

@@ -7,6 +7,15 @@
 
 namespace oztt {
 
+// While it lives, this thread may make calls that are no part of a stream's capture (they wait for no stream and add
+// nothing to one) although one is going on: what a process does once must not fail a capture that happens to be first.
+struct OutsideCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    OutsideCapture() { OZTT_CUDA(cudaThreadExchangeStreamCaptureMode(&mode)); }
+    ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    OutsideCapture(const OutsideCapture&) = delete;
+};
+
 // The word that a bounded wait of a layer product writes when it gives up: host memory that every device reaches. These
 // calls do not wait for their kernels, so the next of them, or the optimiser's call that would use what they computed,
 // looks at it and throws (linear.cu).
@@ -27,6 +36,7 @@ struct DeviceScope {
         static std::atomic<uint64_t> opened{0};
         if (device < 64 && (opened.load() >> device & 1)) return;
         try {
+            OutsideCapture outside;
             open_device(device);
         } catch (...) {
             cudaSetDevice(before);

@@ -31,18 +31,23 @@ namespace oztt {
 // Both of launch.cuh.
 static std::atomic<int*> known_word{nullptr};
 int* error_word() {
-    static std::once_flag once;
-    std::call_once(once, [] {
-        int* word = nullptr;
-        if (cudaHostAlloc(&word, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
-            *word = 0;
-            known_word = word;
-        } else {
-            cudaGetLastError();
-        }
-    });
-    if (!known_word) throw Error(OZTT_ERUNTIME, "linear: no pinned host memory for the error word");
-    return known_word;
+    if (int* word = known_word) return word;
+    static std::mutex mu;
+    std::lock_guard<std::mutex> lock(mu);
+    if (int* word = known_word) return word;
+    int* word = nullptr;
+    cudaError_t failed;
+    {
+        OutsideCapture outside;
+        failed = cudaHostAlloc(&word, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+    }
+    if (failed != cudaSuccess) {  // the next call tries again
+        cudaGetLastError();
+        throw Error(OZTT_ERUNTIME, std::string("linear: no pinned host memory for the error word: ") + cudaGetErrorString(failed));
+    }
+    *word = 0;
+    known_word = word;
+    return word;
 }
 void check_earlier_calls() {
     int* word = known_word;
