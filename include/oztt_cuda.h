@@ -439,8 +439,8 @@ int oztt_get_option(int32_t option, int32_t* value);
  * bits, each result rounded once); asynchronous on `stream`, with scratch from the stream-ordered allocator.
  * Any strides are taken; operands whose rows start on 16 bytes (and outputs whose rows start on 8) are read and
  * written as they lie, others cost a copy of the operand. Outputs must not overlap operands, except y the
- * residual it is computed from. A kernel that gives up a wait is reported by the next call, an optimiser's included
- * (OZTT_ERUNTIME, with nothing done). */
+ * residual it is computed from. A kernel that gives up a wait is reported by the device's next call, an optimiser's
+ * included (OZTT_ERUNTIME, with nothing done), or by oztt_layer_status. */
 enum { OZTT_ACT_NONE = 0, OZTT_ACT_RELU = 1, OZTT_ACT_GELU = 2, OZTT_ACT_GELU_TANH = 3, OZTT_ACT_SILU = 4 };
 
 /* A matrix (or, with row_stride unused, a vector) by its strides in elements; data may be NULL where the
@@ -470,6 +470,10 @@ typedef struct oztt_linear_grad {
     oztt_view dy, pre, x, w, dx, dw, db;
 } oztt_linear_grad;
 int oztt_linear_backward(int device_id, const oztt_linear_grad* args, void* stream, char* err, size_t errlen);
+
+/* OZTT_ERUNTIME, once, if a kernel of an earlier layer product on the device gave up a wait, so that its outputs are not
+ * valid; else OZTT_OK. Waits for nothing: to ask about the last calls, synchronise their stream first. */
+int oztt_layer_status(int device_id, char* err, size_t errlen);
 
 /* ---- AdamW over many tensors -----------------------------------------------------------------------
  * No counterpart in the reference. With g = grad * scale, in 32 bits:

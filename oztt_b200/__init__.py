@@ -32,7 +32,7 @@ __all__ = [
     "Scheme", "Format", "Reconstruction", "Options", "DeviceOptions", "Info", "Context",
     "is_available", "format_name", "IIPlan", "ii_int8_plan", "ii_int8_run", "ii_int8_run_device",
     "lib", "library_path", "linear", "linear_backward",
-    "AdamW",
+    "AdamW", "layer_status",
 ]
 
 _HERE = Path(__file__).resolve().parent
@@ -208,6 +208,7 @@ _SIGNATURES = {
     "oztt_resident_gemm": [_P, _P, _P, _I32, ctypes.POINTER(_COptions), ctypes.POINTER(_CInfo), _ERR, _SZ],
     "oztt_linear_forward": [ctypes.c_int, _P, _P, _ERR, _SZ],
     "oztt_linear_backward": [ctypes.c_int, _P, _P, _ERR, _SZ],
+    "oztt_layer_status": [ctypes.c_int, _ERR, _SZ],
     "oztt_adamw_step": [ctypes.c_int, _P, _U64, _P, _P, _P, _ERR, _SZ],
     "oztt_adamw_values": [ctypes.c_int, _P, _U64, _P, _P, _P, _ERR, _SZ],
     "oztt_set_option": [_I32, _I32, _ERR, _SZ],
@@ -215,6 +216,7 @@ _SIGNATURES = {
     "oztt_is_available": [_I32],
     "oztt_format_name": [_I32],
     "oztt_test_linear_error": [_I32, _ERR, _SZ],
+    "oztt_test_device_error": [ctypes.c_int, _I32, _ERR, _SZ],
     "oztt_test_udiv_small": [ctypes.c_uint32, ctypes.c_uint32],
     "oztt_test_ext80_dot": [_P, _P, _U64, ctypes.c_double],
     "oztt_test_gemm_wait_timeout": [_U64, _P, _P, _ERR, _SZ],
@@ -710,6 +712,12 @@ def get_option(option: int) -> int:
     if rc != OK:
         _raise(rc, "unknown option")
     return v.value
+
+
+def layer_status(device: int = 0) -> None:
+    """Raise RuntimeError, once, if a kernel of an earlier layer product on the device gave up a wait, so that its outputs
+    are not valid. Waits for nothing: synchronise the stream of the last calls first (oztt_layer_status)."""
+    call("oztt_layer_status", device)
 
 
 def call(name: str, *args) -> None:

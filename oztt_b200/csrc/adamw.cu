@@ -459,7 +459,7 @@ static void step(int device, const oztt_adamw_tensor* tensors, uint64_t count, c
     const Moments mo = check_moments(state, some, "adamw");
     if (!some) return;
     DeviceScope scope(device);
-    check_earlier_calls();  // gradients of a product that gave up are not applied
+    check_earlier_calls(device);  // gradients of a product that gave up are not applied
     Hyper h;
     h.beta1 = (float)hp->beta1;
     h.one_minus_beta1 = (float)(1.0 - hp->beta1);
@@ -509,7 +509,7 @@ static void values(int device, const oztt_adamw_moments* state, uint64_t blocks,
     if (!m_out || !v_out || ((reinterpret_cast<uintptr_t>(m_out) | reinterpret_cast<uintptr_t>(v_out)) & 31))
         throw Error(OZTT_EINVAL, "adamw_values: the outputs must be given and 32-byte aligned");
     DeviceScope scope(device);
-    check_earlier_calls();
+    check_earlier_calls(device);
     const uint64_t groups = blocks * (BLOCK / 16);
     const unsigned grid = (unsigned)std::min<uint64_t>((groups + 255) / 256, 148 * 32);
     launch_overlapped(moments_kernel, dim3(grid), 256, 0, dim3(0), st, mo, groups, m_out, v_out);

@@ -16,11 +16,11 @@ struct OutsideCapture {
     OutsideCapture(const OutsideCapture&) = delete;
 };
 
-// The word that a bounded wait of a layer product writes when it gives up: host memory that every device reaches. These
-// calls do not wait for their kernels, so the next of them, or the optimiser's call that would use what they computed,
+// The word that a bounded wait of a layer product writes when it gives up: host memory, a word for each device. These
+// calls do not wait for their kernels, so the device's next call, or the optimiser's that would use what they computed,
 // looks at it and throws (linear.cu).
-int* error_word();
-void check_earlier_calls();
+int* error_word(int device);
+void check_earlier_calls(int device);
 
 // Makes `device` current for one call.
 struct DeviceScope {

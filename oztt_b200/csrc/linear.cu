@@ -29,30 +29,34 @@
 namespace oztt {
 
 // Both of launch.cuh.
-static std::atomic<int*> known_word{nullptr};
-int* error_word() {
-    if (int* word = known_word) return word;
+constexpr int MOST_WORDS = 64;  // devices beyond share the last
+static std::atomic<int*> known_words{nullptr};
+int* error_word(int device) {
     static std::mutex mu;
-    std::lock_guard<std::mutex> lock(mu);
-    if (int* word = known_word) return word;
-    int* word = nullptr;
-    cudaError_t failed;
-    {
-        OutsideCapture outside;
-        failed = cudaHostAlloc(&word, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+    if (!known_words) {
+        std::lock_guard<std::mutex> lock(mu);
+        if (!known_words) {
+            int* words = nullptr;
+            cudaError_t failed;
+            {
+                OutsideCapture outside;
+                failed = cudaHostAlloc(&words, MOST_WORDS * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+            }
+            if (failed != cudaSuccess) {  // the next call tries again
+                cudaGetLastError();
+                throw Error(OZTT_ERUNTIME,
+                            std::string("linear: no pinned host memory for the error words: ") + cudaGetErrorString(failed));
+            }
+            std::fill(words, words + MOST_WORDS, 0);
+            known_words = words;
+        }
     }
-    if (failed != cudaSuccess) {  // the next call tries again
-        cudaGetLastError();
-        throw Error(OZTT_ERUNTIME, std::string("linear: no pinned host memory for the error word: ") + cudaGetErrorString(failed));
-    }
-    *word = 0;
-    known_word = word;
-    return word;
+    return known_words + std::min(device, MOST_WORDS - 1);
 }
-void check_earlier_calls() {
-    int* word = known_word;
-    if (!word) return;  // no product has run
-    if (const int code = __atomic_exchange_n(word, 0, __ATOMIC_RELAXED))
+void check_earlier_calls(int device) {
+    if (device < 0) throw Error(OZTT_EINVAL, "device_id must be nonnegative");
+    if (!known_words) return;  // no product has run
+    if (const int code = __atomic_exchange_n(error_word(device), 0, __ATOMIC_RELAXED))
         throw Error(OZTT_ERUNTIME, "linear: a kernel of an earlier call gave up waiting (code " + std::to_string(code) +
                                        "); that call's outputs are not valid");
 }
@@ -1266,12 +1270,13 @@ static uint64_t padded(uint64_t elements) { return round_up(elements, 64); }
 
 // One call's scratch memory: laid out first, then allocated at once, and the operands' copies made in one launch.
 struct Scratch {
+    int device;
     cudaStream_t st;
     uint64_t bytes = 0;
     DevBuf buf;
     Packs packs;
     uint64_t pack_at[4];
-    explicit Scratch(cudaStream_t s) : st(s), buf(s) { packs.count = 0; }
+    Scratch(int d, cudaStream_t s) : device(d), st(s), buf(s) { packs.count = 0; }
     int64_t reserve(uint64_t size) {
         const uint64_t at = bytes;
         bytes += round_up(std::max<uint64_t>(size, 1), 256);
@@ -1391,7 +1396,7 @@ static uint32_t room_for(Kernel* kernel, uint32_t smem, uint32_t size, std::atom
 }
 
 template <bool HALF, int COUNT, int BQ, int STAGES, int CTAS>
-static void launch_tiles(const Task* tasks, cudaStream_t st) {
+static void launch_tiles(const Task* tasks, int device, cudaStream_t st) {
     constexpr uint32_t SMEM = STAGES * (P_BYTES + BQ * BK * 2) + 256 + 1024;
     static std::atomic<uint64_t> allowed{0};
     auto* kernel = product_kernel<HALF, COUNT, BQ, STAGES, CTAS>;
@@ -1411,17 +1416,17 @@ static void launch_tiles(const Task* tasks, cudaStream_t st) {
     else
         for (uint32_t s = std::min<uint32_t>(8, shortest / 2); s > 1 && split == 1; --s)
             if (ps.tiles * s <= 296 && ps.tiles <= std::max(2 * alone(s), alone((s + 1) / 2))) split = s;
-    launch_overlapped(kernel, dim3(ps.tiles * split), THREADS, SMEM, dim3(split), st, ps, error_word());
+    launch_overlapped(kernel, dim3(ps.tiles * split), THREADS, SMEM, dim3(split), st, ps, error_word(device));
 }
 
 template <bool HALF, int COUNT, int BQ, bool TURNED>
-static void launch_pairs(const Task* tasks, cudaStream_t st) {
+static void launch_pairs(const Task* tasks, int device, cudaStream_t st) {
     constexpr uint32_t SMEM = PAIR_STAGES_BYTES + FINISHERS * PATCH_BYTES + 256 + 1024;
     static std::atomic<uint64_t> allowed{0};
     auto* kernel = pair_product_kernel<HALF, COUNT, BQ, TURNED>;
     allow_smem(kernel, SMEM, allowed);
     const Products<COUNT> ps = describe_all<HALF, COUNT>(tasks, 2 * BP, BQ, BQ / 2, TURNED);
-    launch_overlapped(kernel, dim3(2 * std::min<uint32_t>(ps.tiles, 74)), PAIR_THREADS, SMEM, dim3(0), st, ps, error_word());
+    launch_overlapped(kernel, dim3(2 * std::min<uint32_t>(ps.tiles, 74)), PAIR_THREADS, SMEM, dim3(0), st, ps, error_word(device));
 }
 
 template <bool HALF, int M, bool VEC>
@@ -1557,17 +1562,17 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
     //   512x2048    4096     17.2     15.9     26.1
     if (!empty && rows > 128 && (pair_tiles >= 37 || (pair_tiles >= 24 && blocks <= 24))) {
         if (wide)
-            count == 2 ? launch_pairs<HALF, 2, 256, true>(tasks, st) : launch_pairs<HALF, 1, 256, true>(tasks, st);
+            count == 2 ? launch_pairs<HALF, 2, 256, true>(tasks, scratch.device, st) : launch_pairs<HALF, 1, 256, true>(tasks, scratch.device, st);
         else
-            count == 2 ? launch_pairs<HALF, 2, 256, false>(tasks, st) : launch_pairs<HALF, 1, 256, false>(tasks, st);
+            count == 2 ? launch_pairs<HALF, 2, 256, false>(tasks, scratch.device, st) : launch_pairs<HALF, 1, 256, false>(tasks, scratch.device, st);
     } else if (rows <= 16 && narrow)
-        launch_tiles<HALF, 1, 16, 6, 2>(tasks, st);
+        launch_tiles<HALF, 1, 16, 6, 2>(tasks, scratch.device, st);
     else if (rows <= 32 && narrow)
-        launch_tiles<HALF, 1, 32, 5, 2>(tasks, st);
+        launch_tiles<HALF, 1, 32, 5, 2>(tasks, scratch.device, st);
     else if (rows <= 64 || tiles <= 32 || blocks <= 24)
-        count == 2 ? launch_tiles<HALF, 2, 64, 4, 2>(tasks, st) : launch_tiles<HALF, 1, 64, 4, 2>(tasks, st);
+        count == 2 ? launch_tiles<HALF, 2, 64, 4, 2>(tasks, scratch.device, st) : launch_tiles<HALF, 1, 64, 4, 2>(tasks, scratch.device, st);
     else
-        count == 2 ? launch_tiles<HALF, 2, 128, 3, 2>(tasks, st) : launch_tiles<HALF, 1, 128, 3, 2>(tasks, st);
+        count == 2 ? launch_tiles<HALF, 2, 128, 3, 2>(tasks, scratch.device, st) : launch_tiles<HALF, 1, 128, 3, 2>(tasks, scratch.device, st);
 }
 
 template <bool HALF>
@@ -1622,7 +1627,7 @@ static void forward(int device, const oztt_linear& a, cudaStream_t st) {
     check_output(a.pre, a.m, a.n, "linear: pre");
     if (!some) return;
     DeviceScope scope(device);
-    check_earlier_calls();
+    check_earlier_calls(device);
     Epilogue e{};
     e.rows = a.m;
     e.cols = a.n;
@@ -1633,7 +1638,7 @@ static void forward(int device, const oztt_linear& a, cudaStream_t st) {
     e.bias_stride = a.bias.col_stride;
     e.act = a.activation;
     Task t{{a.w.data, a.n, a.k, a.w.row_stride, a.w.col_stride}, {a.x.data, a.m, a.k, a.x.row_stride, a.x.col_stride}, e};
-    Scratch scratch(st);
+    Scratch scratch(device, st);
     const int count = plan(&t, 1, scratch);
     scratch.allocate();
     run<HALF>(&t, count, scratch, st);
@@ -1654,7 +1659,7 @@ static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
     check_output(a.dw, a.n, a.k, "linear_backward: dw");
     check_output(a.db, 1, a.n, "linear_backward: db");
     DeviceScope scope(device);
-    check_earlier_calls();
+    check_earlier_calls(device);
     const View dy = view(a.dy), z = act ? view(a.pre) : View{};
     const auto fits = [](const View& v) { return !v.p || (v.cs == 1 && v.rs % 8 == 0 && aligned16(v.p)); };
     const bool products = mn && ((a.dx.data && a.k) || (a.dw.data && a.k));
@@ -1670,7 +1675,7 @@ static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
     if (mn && most > 8 * cluster) clusters = std::max<uint64_t>(1, std::min(most / cluster, (148 * 4) / (strips * cluster)));
     if (strips >= (1ull << 31)) throw Error(OZTT_EINVAL, "linear_backward: problem too large");
 
-    Scratch scratch(st);
+    Scratch scratch(device, st);
     const int64_t dz_at = write ? scratch.reserve(a.m * ld * 2) : -1;
     const int64_t sums_at = sum && clusters > 1 ? scratch.reserve(clusters * a.n * 4) : -1;
     const View dz = write ? View{nullptr, (int64_t)ld, 1} : dy;
@@ -1725,7 +1730,13 @@ extern "C" int oztt_linear_backward(int device_id, const oztt_linear_grad* args,
     });
 }
 
+extern "C" int oztt_layer_status(int device_id, char* err, size_t errlen) {
+    return oztt::guarded(err, errlen, [&] { oztt::check_earlier_calls(device_id); });
+}
+
 // Puts a wait's error code where a kernel would have put it, for the test of how the next call reports it.
-extern "C" int oztt_test_linear_error(int32_t code, char* err, size_t errlen) {
-    return oztt::guarded(err, errlen, [&] { *oztt::error_word() = code; });
+extern "C" int oztt_test_device_error(int device_id, int32_t code, char* err, size_t errlen);
+extern "C" int oztt_test_linear_error(int32_t code, char* err, size_t errlen) { return oztt_test_device_error(0, code, err, errlen); }
+extern "C" int oztt_test_device_error(int device_id, int32_t code, char* err, size_t errlen) {
+    return oztt::guarded(err, errlen, [&] { *oztt::error_word(device_id) = code; });
 }
