@@ -120,18 +120,25 @@ class AdamW:
     def state_dict(self) -> dict:
         """What load_state_dict needs to go on from here: the number of steps, the moments as they are kept, and the
         masters. The tensors are the optimiser's own."""
-        d = {"t": self.t, "state_bits": self.state_bits, "seed": self.seed, "m": self._m, "v": self._v,
-             "masters": self.masters}
+        d = {"t": self.t, "state_bits": self.state_bits, "seed": self.seed, "counts": tuple(self._counts), "m": self._m,
+             "v": self._v, "masters": self.masters}
         if self.state_bits == 8:
             d["m_exp"], d["v_exp"] = self._m_exp, self._v_exp
         return d
 
     def load_state_dict(self, d: dict) -> None:
-        """Copies a state_dict of an optimiser of like tensors and bits."""
+        """Copies a state_dict of an optimiser of like tensors and bits; ValueError, with nothing copied, for another."""
         names = ["m", "v"] + (["m_exp", "v_exp"] if self.state_bits == 8 else [])
-        if d.get("state_bits") != self.state_bits or any(d[n].shape != getattr(self, "_" + n).shape for n in names):
+        missing = [n for n in (*names, "masters", "t", "seed") if n not in d]
+        if missing:
+            raise ValueError(f"AdamW: the state has no {', '.join(missing)}")
+        like = lambda x, y: x is None if y is None else (  # noqa: E731
+            torch.is_tensor(x) and x.shape == y.shape and x.dtype == y.dtype)
+        # (a state without counts was saved before they were part of one)
+        if (d.get("state_bits") != self.state_bits or list(d.get("counts", self._counts)) != self._counts
+                or not all(like(d[n], getattr(self, "_" + n)) for n in names)):
             raise ValueError("AdamW: the state is of other tensors or bits")
-        if [w is None for w in d["masters"]] != [w is None for w in self.masters]:
+        if len(d["masters"]) != len(self.masters) or not all(map(like, d["masters"], self.masters)):
             raise ValueError("AdamW: the state has other masters")
         for n in names:
             getattr(self, "_" + n).copy_(d[n])
