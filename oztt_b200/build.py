@@ -4,6 +4,7 @@ Produces
   oztt_b200/liboztt.so            the CUDA kernels for sm_100a, the planner, the C ABI
                                   (include/oztt_cuda.h) and the C++ API (include/ozTTgemm/ozTTgemm.hpp)
   oztt_b200/_torch.so             csrc/torch_binding.cpp: the calls on torch's CUDA tensors over the C ABI
+                                  (where this interpreter has torch)
   oztt_b200/_build/gemm_example   examples/gemm.cpp linked against it
   oztt_b200/_build/correctness    tests/cpp/correctness.cpp linked against it
 Object files go to oztt_b200/_build/. Nothing is installed outside the repository; the built files
@@ -85,13 +86,16 @@ def build_library(force: bool = False) -> Path:
     return LIB
 
 
-def build_torch_binding(force: bool = False) -> Path:
+def build_torch_binding(force: bool = False) -> Path | None:
     """oztt_b200/_torch.so: the binding of the calls on torch's tensors to the C ABI, for the torch of this
-    interpreter."""
+    interpreter; nothing without one, which only those calls need."""
     import importlib.util
     import sysconfig
 
-    torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    found = importlib.util.find_spec("torch")
+    if found is None:
+        return None
+    torch = Path(found.submodule_search_locations[0])
     src = CSRC / "torch_binding.cpp"
     # built again for another torch or Python
     stamp, made_for = OUT / "torch_binding.for", f"{torch} {(torch / 'version.py').read_text()} {sys.version}"
