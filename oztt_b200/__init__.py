@@ -31,9 +31,8 @@ import numpy as np
 __all__ = [
     "Scheme", "Format", "Reconstruction", "Options", "DeviceOptions", "Info", "Context",
     "is_available", "format_name", "IIPlan", "ii_int8_plan", "ii_int8_run", "ii_int8_run_device",
-    "lib", "library_path", "linear", "linear_backward",
-    "AdamW", "layer_status",
-]
+    "lib", "library_path", "layer_status",
+]  # linear, linear_backward and AdamW, which import torch, by name only: a star import needs no torch
 
 _HERE = Path(__file__).resolve().parent
 library_path = _HERE / "liboztt.so"
