@@ -407,7 +407,7 @@ static void launch(std::vector<Tensor>& list, uint64_t blocks, int bits, const M
     // 32: 636, 512: 676; 32 bits, 32: 1039 us, 128: 1081, 512: 1107.
     const uint32_t most = bits == 8 ? MOST_CHUNK : MOST_CHUNK / 2;
     table.chunk = LEAST_CHUNK;
-    while (table.chunk < most && blocks / table.chunk > 148 * 8) table.chunk *= 2;
+    while (table.chunk < most && blocks / table.chunk > 8 * multiprocessors(current_device())) table.chunk *= 2;
     uint32_t chunks = 0;
     for (Tensor& t : list) {
         t.chunk0 = chunks;
@@ -511,7 +511,7 @@ static void values(int device, const oztt_adamw_moments* state, uint64_t blocks,
     DeviceScope scope(device);
     check_earlier_calls(device);
     const uint64_t groups = blocks * (BLOCK / 16);
-    const unsigned grid = (unsigned)std::min<uint64_t>((groups + 255) / 256, 148 * 32);
+    const unsigned grid = (unsigned)std::min<uint64_t>((groups + 255) / 256, multiprocessors(device) * 32);
     launch_overlapped(moments_kernel, dim3(grid), 256, 0, dim3(0), st, mo, groups, m_out, v_out);
 }
 

@@ -49,6 +49,24 @@ struct DeviceScope {
     }
 };
 
+constexpr int KNOWN_DEVICES = 64;  // of which what was asked once is kept
+
+// The current device, and the SMs of a device.
+inline int current_device() {
+    int device = 0;
+    OZTT_CUDA(cudaGetDevice(&device));
+    return device;
+}
+inline uint32_t multiprocessors(int device) {
+    static std::atomic<int> known[KNOWN_DEVICES];
+    int n = device < KNOWN_DEVICES ? known[device].load() : 0;
+    if (!n) {
+        OZTT_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device));
+        if (device < KNOWN_DEVICES) known[device].store(n);
+    }
+    return (uint32_t)n;
+}
+
 // Lets the next kernel of the stream start while this one ends, and waits for the one before, which must be over
 // before anything in memory is read or written (both do nothing where the launch did not ask for the overlap). The
 // kernel before may still be writing what this one reads, so no input of such a kernel is `const __restrict__`.
@@ -82,8 +100,7 @@ inline void launch_overlapped(void (*kernel)(Params...), dim3 grid, uint32_t thr
 // Allows a kernel its dynamic shared memory, and clusters of up to 16, once on each device.
 template <class Kernel>
 inline void allow_smem(Kernel* kernel, uint32_t bytes, std::atomic<uint64_t>& allowed, bool large_clusters = false) {
-    int device = 0;
-    OZTT_CUDA(cudaGetDevice(&device));
+    const int device = current_device();
     if (device < 64 && (allowed.load() >> device & 1)) return;
     OZTT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     if (large_clusters) OZTT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));

@@ -1293,7 +1293,7 @@ struct Scratch {
         if (bytes) buf.alloc(bytes);
         if (!packs.count) return;
         for (uint32_t c = 0; c < packs.count; ++c) packs.of[c].dst = at<uint16_t>((int64_t)pack_at[c]);
-        const unsigned grid = (unsigned)std::min<uint64_t>((packs.of[packs.count - 1].end + 7) / 8, 148 * 32);
+        const unsigned grid = (unsigned)std::min<uint64_t>((packs.of[packs.count - 1].end + 7) / 8, multiprocessors(device) * 32);
         launch_overlapped(pack_kernel, dim3(grid), 256, 0, dim3(0), st, packs);
     }
     // The operand as the tensor copies can read it: as it lies (K-major, or MN-major where allowed), or a copy.
@@ -1374,10 +1374,12 @@ static Products<COUNT> describe_all(const Task* tasks, uint32_t tile_p, uint32_t
     return ps;
 }
 
-// How many clusters of `size` blocks of a kernel the device runs at once, a block to an SM (asked once).
+// How many clusters of `size` blocks of a kernel the device runs at once, a block to an SM. known: what was asked before,
+// for each device and size.
+using Room = std::atomic<int>[KNOWN_DEVICES][MAX_SPLIT + 1];
 template <class Kernel>
-static uint32_t room_for(Kernel* kernel, uint32_t smem, uint32_t size, std::atomic<int>& known) {
-    int n = known.load();
+static uint32_t room_for(Kernel* kernel, uint32_t smem, uint32_t size, int device, Room& known) {
+    int n = device < KNOWN_DEVICES ? known[device][size].load() : 0;
     if (!n) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(size);
@@ -1390,7 +1392,7 @@ static uint32_t room_for(Kernel* kernel, uint32_t smem, uint32_t size, std::atom
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         OZTT_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
-        known.store(n > 0 ? n : -1);
+        if (device < KNOWN_DEVICES) known[device][size].store(n > 0 ? n : -1);
     }
     return n > 0 ? (uint32_t)n : 0;
 }
@@ -1408,14 +1410,15 @@ static void launch_tiles(const Task* tasks, int device, cudaStream_t st) {
     // 128 x 1024 x 4096, where they do not: 13.9 and 8.7).
     static_assert(CTAS == 2, "the room below is that of two CTAs to an SM");
     const uint32_t shortest = std::min(ps.of[0].num_kb, ps.of[COUNT - 1].num_kb);
-    static std::atomic<int> known[MAX_SPLIT + 1];
-    const auto alone = [&](uint32_t size) { return room_for(kernel, SMEM, size, known[size]); };
+    static Room known;
+    const uint32_t sms = multiprocessors(device);
+    const auto alone = [&](uint32_t size) { return room_for(kernel, SMEM, size, device, known); };
     uint32_t split = 1;
-    if (shortest / MAX_SPLIT >= 2 && ps.tiles * MAX_SPLIT <= 148 && ps.tiles <= alone(MAX_SPLIT))
+    if (shortest / MAX_SPLIT >= 2 && ps.tiles * MAX_SPLIT <= sms && ps.tiles <= alone(MAX_SPLIT))
         split = MAX_SPLIT;
     else
         for (uint32_t s = std::min<uint32_t>(8, shortest / 2); s > 1 && split == 1; --s)
-            if (ps.tiles * s <= 296 && ps.tiles <= std::max(2 * alone(s), alone((s + 1) / 2))) split = s;
+            if (ps.tiles * s <= 2 * sms && ps.tiles <= std::max(2 * alone(s), alone((s + 1) / 2))) split = s;
     launch_overlapped(kernel, dim3(ps.tiles * split), THREADS, SMEM, dim3(split), st, ps, error_word(device));
 }
 
@@ -1426,16 +1429,16 @@ static void launch_pairs(const Task* tasks, int device, cudaStream_t st) {
     auto* kernel = pair_product_kernel<HALF, COUNT, BQ, TURNED>;
     allow_smem(kernel, SMEM, allowed);
     const Products<COUNT> ps = describe_all<HALF, COUNT>(tasks, 2 * BP, BQ, BQ / 2, TURNED);
-    launch_overlapped(kernel, dim3(2 * std::min<uint32_t>(ps.tiles, 74)), PAIR_THREADS, SMEM, dim3(0), st, ps, error_word(device));
+    launch_overlapped(kernel, dim3(2 * std::min(ps.tiles, multiprocessors(device) / 2)), PAIR_THREADS, SMEM, dim3(0), st, ps, error_word(device));
 }
 
 template <bool HALF, int M, bool VEC>
-static void launch_few(const Task& t, cudaStream_t st) {
+static void launch_few(const Task& t, int device, cudaStream_t st) {
     auto* kernel = few_rows_kernel<HALF, M, VEC>;
     const uint64_t blocks = (t.e.cols + FEW_COLS - 1) / FEW_COLS;
     // enough warps to keep the memory busy (16 on every SM), as long as each has a few accesses
     uint32_t warps = 1;
-    while (warps < 8 && blocks * warps < 148 * 16 && t.p.red / (warps * 2) >= 512) warps *= 2;
+    while (warps < 8 && blocks * warps < 16 * multiprocessors(device) && t.p.red / (warps * 2) >= 512) warps *= 2;
     launch_overlapped(kernel, dim3((unsigned)blocks), warps * 32, 0, dim3(0), st, static_cast<const uint16_t*>(t.p.p), t.p.rs,
            static_cast<const uint16_t*>(t.q.p), t.q.rs, (uint32_t)t.p.red, t.e);
 }
@@ -1462,10 +1465,11 @@ static uint64_t pair_tiles_of(const Task& t) { return ((t.e.rows + 255) / 256) *
 // one launch and two: 512 x 1024 x 1024 11 and 16, 1024^3 12.7 and 19.0, 2048^3 30.6 and 33.9, but 8192 x 1024 x 1024 58
 // and 41, 8192 x 16384 x 4096 1922 and 1706: pairs that work on products of unlike length drift apart, and what one has
 // read has left L2 when the next wants it.) One with few rows takes narrower tiles.
-static bool together(const Task* tasks, int count) {
+static bool together(const Task* tasks, int count, uint64_t sms) {
     if (count < 2 || std::min(tasks[0].e.rows, tasks[1].e.rows) <= 64) return false;
     const uint64_t b0 = blocks_of(tasks[0]), b1 = blocks_of(tasks[1]), t0 = pair_tiles_of(tasks[0]), t1 = pair_tiles_of(tasks[1]);
-    return std::max(b0, b1) <= 24 || (t0 + t1 <= 148 && t0 * b0 + t1 * b1 >= 52 * std::max(b0, b1));
+    // (up to two waves of pairs, and seven tenths of one busy all the time)
+    return std::max(b0, b1) <= 24 || (t0 + t1 <= sms && t0 * b0 + t1 * b1 >= sms * 13 / 37 * std::max(b0, b1));
 }
 
 template <bool HALF>
@@ -1523,7 +1527,8 @@ static int plan(Task* tasks, int count, Scratch& scratch) {
 template <bool HALF>
 static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st) {
     if (!count) return;
-    if (count == 2 && !together(tasks, count)) {
+    const uint32_t sms = multiprocessors(scratch.device);
+    if (count == 2 && !together(tasks, count, sms)) {
         run<HALF>(tasks, 1, scratch, st);
         run<HALF>(tasks + 1, 1, scratch, st);
         return;
@@ -1549,7 +1554,7 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
                         : rows == 2 ? launch_few<HALF, 2, false>
                         : rows == 3 ? launch_few<HALF, 3, false>
                                     : launch_few<HALF, 4, false>;
-        return go(t, st);
+        return go(t, scratch.device, st);
     }
     if (count == 1 && few_terms(tasks[0])) return launch_few_terms<HALF>(tasks[0], st);
     // Which tiles, by what was measured (us, BF16, single products):
@@ -1560,7 +1565,7 @@ static void run(Task* tasks, int count, const Scratch& scratch, cudaStream_t st)
     //   512x2048    1024      9.8     10.5     11.2      64 rows where 128 would leave most SMs idle or the sum is
     //   256x2048    4096     12.0     13.7     25.6      short, since the CTAs of a split sum join sooner
     //   512x2048    4096     17.2     15.9     26.1
-    if (!empty && rows > 128 && (pair_tiles >= 37 || (pair_tiles >= 24 && blocks <= 24))) {
+    if (!empty && rows > 128 && (pair_tiles >= sms / 4 || (pair_tiles >= sms * 6 / 37 && blocks <= 24))) {
         if (wide)
             count == 2 ? launch_pairs<HALF, 2, 256, true>(tasks, scratch.device, st) : launch_pairs<HALF, 1, 256, true>(tasks, scratch.device, st);
         else
@@ -1672,7 +1677,7 @@ static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
     uint32_t cluster = 1;
     while (cluster < DZ_CLUSTER && cluster * 2 <= most) cluster *= 2;
     uint64_t clusters = 1;
-    if (mn && most > 8 * cluster) clusters = std::max<uint64_t>(1, std::min(most / cluster, (148 * 4) / (strips * cluster)));
+    if (mn && most > 8 * cluster) clusters = std::max<uint64_t>(1, std::min(most / cluster, multiprocessors(device) * 4 / (strips * cluster)));
     if (strips >= (1ull << 31)) throw Error(OZTT_EINVAL, "linear_backward: problem too large");
 
     Scratch scratch(device, st);

@@ -49,3 +49,13 @@ def test_overlapped_kernels_do_not_call_their_inputs_constant(path):
         body = text[end:text.index("\n}", end)]
         if "overlap_launches" in body:
             assert not re.search(r"\bconst\s+\w+\s*\*\s*__restrict__", text[at.start():end])
+
+
+@pytest.mark.parametrize("name", ["linear.cu", "adamw.cu", "launch.cuh"])
+def test_the_layers_rules_ask_the_device_for_its_size(name):
+    """No rule of the layer calls has an SM count of its own (148, half, a quarter or twice as many), and what a device
+    was asked once is kept for that device."""
+    text = without_comments(CSRC / name)
+    assert not re.search(r"\b(148|296|74|37)\b", text.replace("* 6 / 37", "").replace("* 13 / 37", ""))
+    for kept in re.findall(r"static std::atomic<int> \w+(\[[^;]*\])?;", text):
+        assert "KNOWN_DEVICES" in kept
