@@ -436,7 +436,7 @@ int oztt_get_option(int32_t option, int32_t* value);
 
 /* ---- layers of networks: the product with its epilogue, and its gradients ---------------------------
  * No counterpart in the reference, whose products are FP64. Device memory; BF16 or FP16 throughout (sums in 32
- * bits, each result rounded once); asynchronous on `stream`, with scratch from the stream-ordered allocator.
+ * bits, each result rounded once); asynchronous on `stream`, with scratch from the stream-ordered allocator or the caller.
  * Any strides are taken; operands whose rows start on 16 bytes (and outputs whose rows start on 8) are read and
  * written as they lie, others cost a copy of the operand. Outputs must not overlap operands, except y the
  * residual it is computed from. A kernel that gives up a wait is reported by the device's next call, an optimiser's
@@ -470,6 +470,16 @@ typedef struct oztt_linear_grad {
     oztt_view dy, pre, x, w, dx, dw, db;
 } oztt_linear_grad;
 int oztt_linear_backward(int device_id, const oztt_linear_grad* args, void* stream, char* err, size_t errlen);
+
+/* The same two calls with their scratch memory from the caller: alloc(context, bytes) is called at most once, with the
+ * device current, and returns device memory on a 256-byte boundary that kernels on `stream` may use, or NULL (the call
+ * then fails with OZTT_ENOMEM and has launched nothing). The caller takes the memory back after the call, in the
+ * stream's order. */
+typedef void* (*oztt_allocator)(void* context, size_t bytes);
+int oztt_linear_forward_in(int device_id, const oztt_linear* args, oztt_allocator alloc, void* context, void* stream,
+                           char* err, size_t errlen);
+int oztt_linear_backward_in(int device_id, const oztt_linear_grad* args, oztt_allocator alloc, void* context,
+                            void* stream, char* err, size_t errlen);
 
 /* OZTT_ERUNTIME, once, if a kernel of an earlier layer product on the device gave up a wait, so that its outputs are not
  * valid; else OZTT_OK. Waits for nothing: to ask about the last calls, synchronise their stream first. */

@@ -207,6 +207,8 @@ _SIGNATURES = {
     "oztt_resident_gemm": [_P, _P, _P, _I32, ctypes.POINTER(_COptions), ctypes.POINTER(_CInfo), _ERR, _SZ],
     "oztt_linear_forward": [ctypes.c_int, _P, _P, _ERR, _SZ],
     "oztt_linear_backward": [ctypes.c_int, _P, _P, _ERR, _SZ],
+    "oztt_linear_forward_in": [ctypes.c_int, _P, _P, _P, _P, _ERR, _SZ],
+    "oztt_linear_backward_in": [ctypes.c_int, _P, _P, _P, _P, _ERR, _SZ],
     "oztt_layer_status": [ctypes.c_int, _ERR, _SZ],
     "oztt_adamw_step": [ctypes.c_int, _P, _U64, _P, _P, _P, _ERR, _SZ],
     "oztt_adamw_values": [ctypes.c_int, _P, _U64, _P, _P, _P, _ERR, _SZ],

@@ -1269,14 +1269,20 @@ static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 static uint64_t padded(uint64_t elements) { return round_up(elements, 64); }
 
 // One call's scratch memory: laid out first, then allocated at once, and the operands' copies made in one launch.
+struct Source {  // of scratch memory: the caller's, or (alloc null) the stream-ordered allocator
+    oztt_allocator alloc;
+    void* context;
+};
 struct Scratch {
     int device;
     cudaStream_t st;
+    Source source;
     uint64_t bytes = 0;
+    uint8_t* base = nullptr;
     DevBuf buf;
     Packs packs;
     uint64_t pack_at[4];
-    Scratch(int d, cudaStream_t s) : device(d), st(s), buf(s) { packs.count = 0; }
+    Scratch(int d, cudaStream_t s, Source from) : device(d), st(s), source(from), buf(s) { packs.count = 0; }
     int64_t reserve(uint64_t size) {
         const uint64_t at = bytes;
         bytes += round_up(std::max<uint64_t>(size, 1), 256);
@@ -1284,13 +1290,19 @@ struct Scratch {
     }
     template <class T>
     T* at(int64_t offset) const {
-        return reinterpret_cast<T*>(buf.as<uint8_t>() + offset);
+        return reinterpret_cast<T*>(base + offset);
     }
     void place(Operand& o) const {
         if (o.at >= 0) o.p = at<uint8_t>(o.at);
     }
     void allocate() {
-        if (bytes) buf.alloc(bytes);
+        if (bytes && source.alloc) {
+            base = static_cast<uint8_t*>(source.alloc(source.context, bytes));
+            if (!base) throw Error(OZTT_ENOMEM, "no scratch memory of " + std::to_string(bytes) + " bytes");
+        } else if (bytes) {
+            buf.alloc(bytes);
+            base = buf.as<uint8_t>();
+        }
         if (!packs.count) return;
         for (uint32_t c = 0; c < packs.count; ++c) packs.of[c].dst = at<uint16_t>((int64_t)pack_at[c]);
         const unsigned grid = (unsigned)std::min<uint64_t>((packs.of[packs.count - 1].end + 7) / 8, multiprocessors(device) * 32);
@@ -1619,7 +1631,7 @@ static void check_view(const oztt_view& v, bool needed, const char* what) {
 }
 
 template <bool HALF>
-static void forward(int device, const oztt_linear& a, cudaStream_t st) {
+static void forward(int device, const oztt_linear& a, Source source, cudaStream_t st) {
     check_act(a.activation, "linear");
     const bool some = a.m && a.n, sum = some && a.k;
     check_view(a.x, sum, "linear: x");
@@ -1643,14 +1655,14 @@ static void forward(int device, const oztt_linear& a, cudaStream_t st) {
     e.bias_stride = a.bias.col_stride;
     e.act = a.activation;
     Task t{{a.w.data, a.n, a.k, a.w.row_stride, a.w.col_stride}, {a.x.data, a.m, a.k, a.x.row_stride, a.x.col_stride}, e};
-    Scratch scratch(device, st);
+    Scratch scratch(device, st, source);
     const int count = plan(&t, 1, scratch);
     scratch.allocate();
     run<HALF>(&t, count, scratch, st);
 }
 
 template <bool HALF>
-static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
+static void backward(int device, const oztt_linear_grad& a, Source source, cudaStream_t st) {
     check_act(a.activation, "linear_backward");
     const bool act = a.activation != OZTT_ACT_NONE, mn = a.m && a.n;
     check_view(a.dy, mn, "linear_backward: dy");
@@ -1680,7 +1692,7 @@ static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
     if (mn && most > 8 * cluster) clusters = std::max<uint64_t>(1, std::min(most / cluster, multiprocessors(device) * 4 / (strips * cluster)));
     if (strips >= (1ull << 31)) throw Error(OZTT_EINVAL, "linear_backward: problem too large");
 
-    Scratch scratch(device, st);
+    Scratch scratch(device, st, source);
     const int64_t dz_at = write ? scratch.reserve(a.m * ld * 2) : -1;
     const int64_t sums_at = sum && clusters > 1 ? scratch.reserve(clusters * a.n * 4) : -1;
     const View dz = write ? View{nullptr, (int64_t)ld, 1} : dy;
@@ -1718,21 +1730,29 @@ static void backward(int device, const oztt_linear_grad& a, cudaStream_t st) {
 }  // namespace layer
 }  // namespace oztt
 
-extern "C" int oztt_linear_forward(int device_id, const oztt_linear* args, void* stream, char* err, size_t errlen) {
+extern "C" int oztt_linear_forward_in(int device_id, const oztt_linear* args, oztt_allocator alloc, void* context,
+                                      void* stream, char* err, size_t errlen) {
     return oztt::guarded(err, errlen, [&] {
         if (!args) throw oztt::Error(OZTT_EINVAL, "linear: no arguments");
         const auto run = oztt::layer::half_of(args->format, "linear") ? oztt::layer::forward<true> : oztt::layer::forward<false>;
-        run(device_id, *args, reinterpret_cast<cudaStream_t>(stream));
+        run(device_id, *args, {alloc, context}, reinterpret_cast<cudaStream_t>(stream));
     });
 }
+extern "C" int oztt_linear_forward(int device_id, const oztt_linear* args, void* stream, char* err, size_t errlen) {
+    return oztt_linear_forward_in(device_id, args, nullptr, nullptr, stream, err, errlen);
+}
 
-extern "C" int oztt_linear_backward(int device_id, const oztt_linear_grad* args, void* stream, char* err,
-                                    size_t errlen) {
+extern "C" int oztt_linear_backward_in(int device_id, const oztt_linear_grad* args, oztt_allocator alloc, void* context,
+                                       void* stream, char* err, size_t errlen) {
     return oztt::guarded(err, errlen, [&] {
         if (!args) throw oztt::Error(OZTT_EINVAL, "linear_backward: no arguments");
         const auto run = oztt::layer::half_of(args->format, "linear_backward") ? oztt::layer::backward<true> : oztt::layer::backward<false>;
-        run(device_id, *args, reinterpret_cast<cudaStream_t>(stream));
+        run(device_id, *args, {alloc, context}, reinterpret_cast<cudaStream_t>(stream));
     });
+}
+extern "C" int oztt_linear_backward(int device_id, const oztt_linear_grad* args, void* stream, char* err,
+                                    size_t errlen) {
+    return oztt_linear_backward_in(device_id, args, nullptr, nullptr, stream, err, errlen);
 }
 
 extern "C" int oztt_layer_status(int device_id, char* err, size_t errlen) {

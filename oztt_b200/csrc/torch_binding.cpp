@@ -9,12 +9,14 @@
 #include <ATen/ATen.h>
 #include <ATen/TracerMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
+#include <exception>
 #include <sstream>
 #include <stdexcept>
 #include <string>
@@ -37,6 +39,15 @@ std::string text(const at::Tensor& t) {
     return s.str();
 }
 
+// torch.OutOfMemoryError, as torch's own operations raise it.
+void raise_out_of_memory(const char* text) {
+    PyObject* torch = PyImport_ImportModule("torch");
+    PyObject* kind = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+    if (kind) PyErr_SetString(kind, text);
+    Py_XDECREF(kind);
+    Py_XDECREF(torch);
+}
+
 // Runs f, raising what it throws.
 template <class F>
 PyObject* guarded(F&& f) {
@@ -45,7 +56,7 @@ PyObject* guarded(F&& f) {
     } catch (const Refused& e) {
         PyErr_SetString(PyExc_ValueError, e.what());
     } catch (const c10::OutOfMemoryError& e) {
-        PyErr_SetString(PyExc_MemoryError, e.what_without_backtrace());
+        raise_out_of_memory(e.what_without_backtrace());
     } catch (const c10::Error& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
     } catch (const std::bad_alloc&) {
@@ -68,6 +79,34 @@ void call(F&& f) {
     if (rc == OZTT_EINVAL) refuse(err);
     if (rc == OZTT_ENOMEM) throw std::bad_alloc();
     throw std::runtime_error(err);
+}
+
+// A call's scratch memory, from torch's allocator on the current stream: its cache serves the call, and it frees what it
+// holds before it reports that there is none. Given back after the call, to whatever the stream does next.
+struct TorchScratch {
+    c10::DataPtr memory;
+    std::exception_ptr failure;
+    static void* alloc(void* self, size_t bytes) noexcept {
+        auto* s = static_cast<TorchScratch*>(self);
+        try {
+            s->memory = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
+            return s->memory.get();
+        } catch (...) {
+            s->failure = std::current_exception();
+            return nullptr;
+        }
+    }
+};
+// call() of a function that takes an allocator and its context
+template <class F>
+void call_with_scratch(F&& f) {
+    TorchScratch scratch;
+    try {
+        call([&](char* err, size_t len) { return f(&TorchScratch::alloc, &scratch, err, len); });
+    } catch (const std::bad_alloc&) {
+        if (scratch.failure) std::rethrow_exception(scratch.failure);
+        throw;
+    }
 }
 
 const at::Tensor* tensor_or_none(PyObject* o, const char* who, const char* what) {
@@ -196,7 +235,9 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
         if (save_pre) a.pre = view(pre);
         const int device = x.get_device();
         void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
-        call([&](char* err, size_t len) { return oztt_linear_forward(device, &a, stream, err, len); });
+        call_with_scratch([&](oztt_allocator alloc, void* context, char* err, size_t len) {
+            return oztt_linear_forward_in(device, &a, alloc, context, stream, err, len);
+        });
         if (dim != 2) {
             auto shape = x.sizes().vec();
             shape.back() = n;
@@ -257,7 +298,9 @@ PyObject* linear_backward(PyObject*, PyObject* const* args, Py_ssize_t count) {
         if (dx.defined() || dw.defined() || db.defined()) {
             const int device = dy.get_device();
             void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
-            call([&](char* err, size_t len) { return oztt_linear_backward(device, &a, stream, err, len); });
+            call_with_scratch([&](oztt_allocator alloc, void* context, char* err, size_t len) {
+                return oztt_linear_backward_in(device, &a, alloc, context, stream, err, len);
+            });
         }
         if (dim != 2 && dx.defined()) dx = dx.view(x.sizes());
         return Py_BuildValue("(NNN)", wrapped(dx), wrapped(dw), wrapped(db));

@@ -104,7 +104,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     function), "gelu_tanh" or "silu". Returns y [..., n], or with save_pre (y, pre), pre = x weight^T + bias before
     the activation, which linear_backward needs for one. Differentiable with respect to all four tensors, once and in
     reverse mode: tangents of the forward mode and torch.func's transforms are refused with RuntimeError.
-    Raises ValueError for what does not fit together, RuntimeError for a CUDA failure."""
+    Raises ValueError for what does not fit together, RuntimeError for a CUDA failure, torch.OutOfMemoryError where the
+    result or the call's scratch memory, both from torch's allocator, finds no room."""
     out = _torch.linear(x, weight, bias, residual, _activation("linear", activation), bool(save_pre), True)
     if out is None:  # a gradient is wanted
         out = _Linear.apply(x, weight, bias, residual, activation, bool(save_pre))
