@@ -1003,9 +1003,9 @@ __global__ void __launch_bounds__(256)
 // out[i][j] = the sum of up to T products, for dw of a few tokens, whose output the tiles of the tensor cores finish at
 // 3.9 TB/s at most. Up to 4 terms are bound by the stores, more by the products on the 32-bit pipe. A warp keeps 256
 // columns of P (8 a lane, contiguous) in registers and walks down 8 or 16 rows, one 16-byte store a lane and row, the
-// terms' factors of a row read from shared memory. 4480 x 8576 from 2, 4 and 8 terms: 12.3, 12.3 and 21.7 us (stores alone
-// 10.6, at 7.3 TB/s), by tiles 24; 1024 x 1024 2.2, 2.3 and 3.9, by tiles 6.7; 8192 x 8192 from 8 38.9, by tiles 35. 8 terms
-// with 8 rows a warp: 24.9; with 4 columns a lane 23.9.
+// terms' factors of a row read from shared memory. 4480 x 8576 from 2, 4 and 8 terms: 12.3, 12.6 and 22.8 us (stores
+// alone 10.6, at 7.3 TB/s), by tiles 24; 1024 x 1024 2.3, 2.1 and 3.9, by tiles 6.7. 8 terms with 8 rows a warp take 15 %
+// longer, with 4 columns a lane 10 %.
 template <int T>
 constexpr uint32_t TERM_ROWS = T > 4 ? 16 : 8;
 template <bool HALF, int T>
@@ -1464,11 +1464,14 @@ static bool takes_vectors(const Task& t) {
 static bool few_rows(const Task& t) {
     return t.p.red && t.p.ks == 1 && t.q.ks == 1 && (t.e.rows == 1 || (t.e.rows <= 4 && !takes_vectors(t)));
 }
-// A sum of up to 8 terms without an epilogue, over columns that P has side by side, goes to the kernel for those.
+// A sum of up to 8 terms without an epilogue, over columns that P has side by side, goes to the kernel for those; one of 7
+// or 8 as long as the output is below 40 million elements (us, here and by tiles: 8 terms 4096 x 4096 12.1 and 12.6,
+// 4480 x 8576 22.8 and 23.9, 6144 x 6144 22.5 and 21.7, 8192 x 8192 38.4 and 34.4, 12288 x 12288 77.0 and 74.5; 6 terms
+// 35.2 and 35.1 at 8192 x 8192, 71.2 and 74.5 at 12288 x 12288).
 static bool few_terms(const Task& t) {
     const Epilogue& e = t.e;
-    return t.p.red && t.p.red <= 8 && t.p.mn && e.vec >= 8 && e.cols % 8 == 0 && e.rows <= 65535 * 64 &&
-           e.act == OZTT_ACT_NONE && !e.bias && !e.pre.p && !e.res.p;
+    return t.p.red && (t.p.red <= 6 || (t.p.red <= 8 && e.rows * e.cols < 40000000)) && t.p.mn && e.vec >= 8 &&
+           e.cols % 8 == 0 && e.rows <= 65535 * 64 && e.act == OZTT_ACT_NONE && !e.bias && !e.pre.p && !e.res.p;
 }
 static uint64_t blocks_of(const Task& t) { return (t.p.red + BK - 1) / BK; }
 static uint64_t pair_tiles_of(const Task& t) { return ((t.e.rows + 255) / 256) * ((t.e.cols + 255) / 256); }
