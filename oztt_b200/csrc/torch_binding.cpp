@@ -330,8 +330,9 @@ void refuse_recorders(const char* who) {
     using c10::impl::TorchDispatchModeKey;
     using c10::impl::TorchDispatchModeTLS;
     bool some = at::tracer::impl::is_dispatch_enabled();
-    for (const auto key : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
-        some = some || TorchDispatchModeTLS::get_mode(key).has_value();
+    if (c10::impl::dispatch_mode_enabled())
+        for (const auto key : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+            some = some || TorchDispatchModeTLS::get_mode(key).has_value();
     if (some) throw std::runtime_error(std::string(who) + " cannot be traced or recorded");
 }
 
