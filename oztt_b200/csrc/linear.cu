@@ -91,8 +91,8 @@ struct Epilogue {
 
 // ---- activations in 32 bits ----------------------------------------------------------------------
 // On pairs of values (one instruction of the packed FP32 pipe each), with the two special functions 2^x and 1/x by
-// the hardware's approximations (2^-22): a pass over dz issues 10 instructions an element so, 26 with scalar ones. Only
-// those two flush: a factor 2^x below 2^-126 is zero, so results below |z| 2^-126 in size may be too. Sums, biases,
+// the hardware's approximations (2^-22): a pass over dz issues 11 (SILU) to 18 (GELU) instructions an element so, with
+// scalar ones more than twice as many. Only those two flush: a factor 2^x below 2^-126 is zero, so results below |z| 2^-126 in size may be too. Sums, biases,
 // residuals and products keep subnormal values, as the tensor cores do.
 __device__ __forceinline__ f32x2 exp2_2(f32x2 x) {
     float a, b;
@@ -155,16 +155,6 @@ __device__ __forceinline__ f32x2 activate2(f32x2 z) {
     }
     return z;
 }
-// Both values within [-64, 64], NaN kept.
-__device__ __forceinline__ f32x2 within_64(f32x2 x) {
-    float a, b;
-    unpk2(x, a, b);
-    asm("min.NaN.f32 %0, %0, 0f42800000;" : "+f"(a));
-    asm("min.NaN.f32 %0, %0, 0f42800000;" : "+f"(b));
-    asm("max.NaN.f32 %0, %0, 0fC2800000;" : "+f"(a));
-    asm("max.NaN.f32 %0, %0, 0fC2800000;" : "+f"(b));
-    return pk2(a, b);
-}
 // dz of a pair: dy times the activation's derivative at z.
 template <int ACT>
 __device__ __forceinline__ f32x2 through_slope2(f32x2 dy, f32x2 z) {
@@ -177,20 +167,19 @@ __device__ __forceinline__ f32x2 through_slope2(f32x2 dy, f32x2 z) {
         f32x2 e;
         const f32x2 c = normal_cdf2(z, e);
         return times2(dy, fused2(times2(z, splat2(0.3989422804014327f)), e, c));
-    } else if constexpr (ACT == OZTT_ACT_GELU_TANH || ACT == OZTT_ACT_SILU) {
-        // z s(u) with s the logistic function: s + z u' s (1 - s) = s (1 + z u' (1 - s))
-        f32x2 s, zu;
-        if constexpr (ACT == OZTT_ACT_SILU) {
-            s = logistic2(times2(z, splat2(-kLog2e)));
-            zu = z;
-        } else {
-            constexpr float c = -2.0f * kTanhScale * kLog2e;
-            z = within_64(z);  // the slope is 0 or 1 long before; the cube below would leave the range from 1.2e13 on
-            const f32x2 zz = times2(z, z);
-            s = logistic2(times2(z, fused2(splat2(c * kTanhCube), zz, splat2(c))));
-            zu = times2(z, fused2(splat2(6.0f * kTanhScale * kTanhCube), zz, splat2(2.0f * kTanhScale)));
-        }
-        return times2(times2(dy, s), fused2(zu, sub2(splat2(1.0f), s), splat2(1.0f)));
+    } else if constexpr (ACT == OZTT_ACT_SILU) {
+        // z s(z) with s the logistic function: s + z s (1 - s) = s (1 + z (1 - s))
+        const f32x2 s = logistic2(times2(z, splat2(-kLog2e)));
+        return times2(times2(dy, s), fused2(z, sub2(splat2(1.0f), s), splat2(1.0f)));
+    } else if constexpr (ACT == OZTT_ACT_GELU_TANH) {
+        // z s(u): s + z u' s (1 - s), u' = a + b z^2, summed as s + a t + b z (z t) with t = z s (1 - s), which is zero long
+        // before a power of z alone would leave the range. (db of 8192 x 16384: 104 us, 99 with the powers first, whose
+        // products are NaN from 1.2e13 on; 105 and 107 with z or z^2 cut off by scalar instructions.)
+        constexpr float c = -2.0f * kTanhScale * kLog2e;
+        const f32x2 s = logistic2(times2(z, fused2(splat2(c * kTanhCube), times2(z, z), splat2(c))));
+        const f32x2 t = times2(z, times2(s, sub2(splat2(1.0f), s)));
+        const f32x2 slope = fused2(splat2(2.0f * kTanhScale), t, s);
+        return times2(dy, fused2(splat2(6.0f * kTanhScale * kTanhCube), times2(z, times2(z, t)), slope));
     }
     return dy;
 }
@@ -1132,8 +1121,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs
 // distributed shared memory: into db where one cluster covers all rows, else into partial[cluster][n] for db_kernel.
 // (db and partial may be null.) Bound by memory, which many warps with few accesses each keep busier than few with
 // many: 8192 x 16384 BF16, one read for db alone: 42 us with 8 blocks on an SM and one row ahead, 61 us with 2 and
-// four (41 at the rate of a copy); two reads with gelu_tanh: 99 us with 4 blocks and two rows ahead, 157 with 2 and
-// four (82); strips of 64 columns take 6 % longer with RELU.
+// four (41 at the rate of a copy); two reads with gelu_tanh: 104 us with 4 blocks and two rows ahead, half as
+// long again with 2 and four (82); strips of 64 columns take 6 % longer with RELU.
 constexpr uint32_t DZ_COLS = 128, DZ_ROWS = 16, DZ_CLUSTER = 8;
 constexpr uint32_t DZ_LANES = DZ_COLS / 8;
 template <bool HALF, bool VEC, int ACT>
