@@ -503,7 +503,7 @@ enum { OZTT_TYPE_BF16 = 0, OZTT_TYPE_FP16 = 1, OZTT_TYPE_FP32 = 2 };
 typedef struct oztt_adamw_tensor {
     void* param;
     const void* grad;  /* NULL: the tensor, its moments included, stays as it is */
-    float* master;     /* optional: the step is taken on this copy, and param receives its rounding */
+    float* master;     /* optional: the step is taken on this copy, and param receives its rounding (FP32: its value) */
     uint64_t count;    /* contiguous elements */
     int32_t param_type, grad_type; /* OZTT_TYPE_* */
 } oztt_adamw_tensor;
