@@ -1288,6 +1288,7 @@ struct Scratch {
         if (bytes && source.alloc) {
             base = static_cast<uint8_t*>(source.alloc(source.context, bytes));
             if (!base) throw Error(OZTT_ENOMEM, "no scratch memory of " + std::to_string(bytes) + " bytes");
+            if (reinterpret_cast<uintptr_t>(base) & 255) throw Error(OZTT_EINVAL, "scratch memory must start on 256 bytes");
         } else if (bytes) {
             buf.alloc(bytes);
             base = buf.as<uint8_t>();

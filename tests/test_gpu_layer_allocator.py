@@ -50,6 +50,19 @@ def test_no_memory(oztt, cuda):
         assert all(bool((t == 7).all()) for t in got)
 
 
+def test_memory_off_its_boundary(oztt, cuda):
+    room = torch.empty(1 << 22, dtype=torch.uint8, device="cuda")
+    for name, args, got, want, needs in calls(oztt, 1):
+        for t in got:
+            t.fill_(7)
+        for off in (1, 8, 16, 128):
+            with pytest.raises(ValueError, match="256"):
+                oztt.call(name, 0, args, ALLOCATOR(lambda context, size: room.data_ptr() + off), None,
+                          torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert all(bool((t == 7).all()) for t in got)
+
+
 def test_refusals(oztt, cuda):
     for name in ("oztt_linear_forward_in", "oztt_linear_backward_in"):
         with pytest.raises(ValueError, match="no arguments"):
