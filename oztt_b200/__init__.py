@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import ctypes
 import enum
+import importlib.util
 from dataclasses import dataclass, field
 from pathlib import Path
 
@@ -32,7 +33,7 @@ __all__ = [
     "Scheme", "Format", "Reconstruction", "Options", "DeviceOptions", "Info", "Context",
     "is_available", "format_name", "IIPlan", "ii_int8_plan", "ii_int8_run", "ii_int8_run_device",
     "lib", "library_path", "layer_status",
-]  # linear, linear_backward and AdamW, which import torch, by name only: a star import needs no torch
+]
 
 _HERE = Path(__file__).resolve().parent
 library_path = _HERE / "liboztt.so"
@@ -260,14 +261,14 @@ def _lib() -> ctypes.CDLL:
 
 # What lives in modules that need torch, imported on first use.
 _TORCH_NAMES = {"linear": "layers", "linear_backward": "layers", "AdamW": "optim"}
+if (_HERE / "_torch.so").exists() and importlib.util.find_spec("torch") is not None:  # a star import needs no torch
+    __all__ += _TORCH_NAMES
 
 
 def __getattr__(name: str):
     if name == "lib":
         return _lib()
     if name in _TORCH_NAMES:
-        import importlib
-
         value = getattr(importlib.import_module(f".{_TORCH_NAMES[name]}", __name__), name)
         globals()[name] = value
         return value
