@@ -70,8 +70,9 @@ inline uint32_t multiprocessors(int device) {
 // Lets the next kernel of the stream start while this one ends, and waits for the one before, which must be over
 // before anything in memory is read or written (both do nothing where the launch did not ask for the overlap). The
 // kernel before may still be writing what this one reads, so no input of such a kernel is `const __restrict__`.
-__device__ __forceinline__ void overlap_launches() {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+// early: false to let the next kernel start only when this one has ended.
+__device__ __forceinline__ void overlap_launches(bool early = true) {
+    if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 

@@ -682,7 +682,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     cluster_sync();  // the peer's barriers are initialised before anything is signalled across the pair
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    overlap_launches();
+    // With idle pairs' SMs on the device, the next kernel starts when this one ends: its blocks would all find room on those
+    // SMs and share them, where they could have the whole device a moment later (backward pass of 777 x 1535 x 1001 and the
+    // next call's: 25.6 us, 29.6 when they may start early; with every SM taken 1 to 2 us the other way).
+    overlap_launches(2 * ps.tiles > gridDim.x);
 
     if (warp == 0) {
         if (lane == 0) {
