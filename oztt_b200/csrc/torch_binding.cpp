@@ -336,19 +336,12 @@ void refuse_recorders(const char* who) {
     if (some) throw std::runtime_error(std::string(who) + " cannot be traced or recorded");
 }
 
-// The items of a list or tuple of n, held for the call: another thread may change the list while the lock is released.
-struct Items {
-    PyObject* held;
-    Items(PyObject* o, Py_ssize_t n, const char* what) {
-        if (!PyList_Check(o) && !PyTuple_Check(o)) refuse(std::string("AdamW: ") + what + " must be a list or a tuple");
-        if (PySequence_Fast_GET_SIZE(o) != n) refuse(std::string("AdamW: ") + what + " must be as many as params");
-        held = PySequence_Tuple(o);
-        if (!held) throw std::bad_alloc();
-    }
-    ~Items() { Py_DECREF(held); }
-    Items(const Items&) = delete;
-    PyObject* operator[](Py_ssize_t i) const { return PyTuple_GET_ITEM(held, i); }
-};
+// The items of a list or tuple of n (not to be looked at after the lock has been released).
+PyObject** items(PyObject* o, Py_ssize_t n, const char* what) {
+    if (!PyList_Check(o) && !PyTuple_Check(o)) refuse(std::string("AdamW: ") + what + " must be a list or a tuple");
+    if (PySequence_Fast_GET_SIZE(o) != n) refuse(std::string("AdamW: ") + what + " must be as many as params");
+    return PySequence_Fast_ITEMS(o);
+}
 
 // The record of the moments (m, v, m_exp, v_exp) of `blocks` blocks, the exponents None with 32 bits. Their addresses
 // are asked for in every call: a copy of an optimiser has other buffers than the original.
@@ -384,7 +377,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
         refuse_recorders("AdamW.step");
         auto* t = static_cast<oztt_adamw_tensor*>(table.buf);
         const Py_ssize_t n = table.len / (Py_ssize_t)sizeof(oztt_adamw_tensor);
-        const Items params(args[1], n, "params"), masters(args[2], n, "masters"), grads(args[3], n, "grads");
+        PyObject **params = items(args[1], n, "params"), **masters = items(args[2], n, "masters"),
+                 **grads = items(args[3], n, "grads");
         const int device = (int)PyLong_AsLong(args[7]);
         uint64_t blocks = 0;
         for (Py_ssize_t i = 0; i < n; ++i) blocks += (t[i].count + OZTT_ADAMW_BLOCK - 1) / OZTT_ADAMW_BLOCK;
@@ -419,8 +413,6 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
                 refuse("AdamW: grad_scale must be one FP32 number on the parameters' device");
             hyper.grad_scale = s->const_data_ptr<float>();
         }
-        void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
-        call([&](char* err, size_t len) { return oztt_adamw_step(device, t, (uint64_t)n, &moments, &hyper, stream, err, len); });
         // what was saved for a backward pass that has not run is no longer what it was
         const auto written = [](PyObject* o) {
             if (o == Py_None) return;
@@ -433,6 +425,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t count) {
             written(masters[i]);
         }
         for (Py_ssize_t i = 0; i < 4; ++i) written(PyTuple_GET_ITEM(args[5], i));
+        void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+        call([&](char* err, size_t len) { return oztt_adamw_step(device, t, (uint64_t)n, &moments, &hyper, stream, err, len); });
         Py_RETURN_NONE;
     });
     PyBuffer_Release(&table);
